@@ -161,6 +161,94 @@ int vx_fsq(vx_ctx* ctx, const uint16_t* w_in, const float* b_in, const uint16_t*
            int in_dim, int latent_dim, int out_dim, float scale, const float* hidden, int rows, float* out,
            vx_stream stream);
 
+/* ----------------------------------------------------------------- 4-bit KV cache */
+
+/* A KV cache held in 4 bits, for decoding long sequences (no counterpart in the reference,
+ * whose StaticKvCache is f32: minicpm4/cache.rs).  A key or value row of d = head_dim numbers
+ * (post-RoPE keys, as in StaticKvCache) is d / 2 bytes of e2m1 codes, dim 2j in the low nibble
+ * of byte j, and d / 16 e4m3 scales, one for each 16 dims: value = code * scale, 72 B a row at
+ * d = 128 for 512 B of f32.  The buffers are the caller's device memory:
+ *   k_codes, v_codes    [batch, n_kv_heads, capacity, head_dim / 2]
+ *   k_scales, v_scales  [batch, n_kv_heads, capacity, head_dim / 16]
+ *   weights             [batch, n_kv_heads, capacity] f32 or NULL: the attention that each row
+ *                       has received, summed (vx_kv4_attend with track)
+ *   positions           [batch, n_kv_heads, capacity] int64 or NULL: the token position of each row
+ * head_dim is 64 or 128, capacity a multiple of 32, codes and scales are 16-byte aligned.
+ * How many rows of a sequence are filled is the caller's: device int32 arrays of `batch`
+ * lengths, so that a captured graph can be replayed at other lengths.  Lengths outside their
+ * range are found on the device: the sequence is left as it was (vx_kv4_attend: its output is
+ * NaN) and the next vx_ctx_synchronize reports VX_ERR_ARG.  Calls that write a cache and calls
+ * that read it are ordered by the caller (one stream, or events). */
+typedef struct {
+  uint8_t* k_codes;
+  uint8_t* k_scales;
+  uint8_t* v_codes;
+  uint8_t* v_scales;
+  float* weights;
+  int64_t* positions;
+  int batch;
+  int n_kv_heads;
+  int capacity;
+  int head_dim;
+} vx_kv4;
+
+/* Quantise the rows of new tokens into the cache: token i < counts[b] of sequence b (counts
+ * NULL: S) goes into slot start[b] + i of every KV head.  k, v: element (b, i, head, dim) at
+ * b * batch_stride + i * token_stride + head * head_dim + dim (f32, strides in elements and
+ * multiples of 4), so the rows may lie in a fused q | k | v projection.  A group's scale is
+ * e4m3(amax / 6), a code e2m1(x / scale), each to nearest with ties to even; values beyond
+ * 6 * 448 saturate, and a group that holds a NaN reads back as NaN.  The rows' weights become
+ * 0 and their positions first_position[b] + i (NULL: the slot), where the cache keeps them. */
+int vx_kv4_append(vx_ctx* ctx, const vx_kv4* cache, const float* k, const float* v, int64_t batch_stride,
+                  int64_t token_stride, int S, const int32_t* start, const int32_t* counts,
+                  const int32_t* first_position, vx_stream stream);
+/* The values of rows start[b] .. start[b] + counts[b] (start NULL: 0, counts NULL: n; counts[b]
+ * <= n) as k, v [batch, n_kv_heads, n, head_dim] f32; rows past counts[b] are 0. */
+int vx_kv4_read(vx_ctx* ctx, const vx_kv4* cache, int n, const int32_t* start, const int32_t* counts, float* k,
+                float* v, vx_stream stream);
+/* Attention of one query token per sequence over its first lens[b] rows (as
+ * vx_attention_decode over an f32 cache): q [batch] rows of nh * head_dim f32, q_stride
+ * elements apart (16-byte aligned), query head h on KV head h / (nh / n_kv_heads); out likewise.
+ * 0 <= lens[b] <= max_len; a sequence of length 0 gives zeros.  With track every row's weight
+ * grows by the probabilities that it received from the query heads of its KV head.  The
+ * workspace (16-byte aligned, vx_kv4_attend_workspace bytes, may be NULL for 0) is this call's
+ * alone until it has run: calls and captured graphs that may overlap need one each. */
+size_t vx_kv4_attend_workspace(const vx_kv4* cache, int nh, int max_len, int track);
+int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* cache, const float* q, int64_t q_stride, int nh, const int32_t* lens,
+                  int max_len, float scale, int track, float* out, int64_t out_stride, void* workspace,
+                  size_t workspace_bytes, vx_stream stream);
+/* Let go of rows by accumulated weight: of the lens[b] <= max_len (<= 131072) rows of each KV
+ * head the `keep` of largest weight stay (ties: the lowest slots; a NaN counts as the largest),
+ * rows of a position below `sink` or not below seen[b] - recent before all others (seen[b]: the
+ * tokens that the sequence has had; sink + recent <= keep).  Rows that stay below slot `keep`
+ * stay where they are; the i-th free slot there takes the i-th kept row behind it, with its
+ * weight and position (attention does not depend on the order of rows).  weights_out and
+ * positions_out [batch, n_kv_heads, capacity] receive the kept rows' (they may be the cache's
+ * own; entries past the new length are left as they were); lens_out (not lens) receives
+ * min(lens[b], keep). */
+int vx_kv4_evict(vx_ctx* ctx, const vx_kv4* cache, const int32_t* lens, const int32_t* seen, int max_len, int keep,
+                 int sink, int recent, float* weights_out, int64_t* positions_out, int32_t* lens_out,
+                 vx_stream stream);
+
+/* ----------------------------------------------------------------- sampling */
+
+/* One token id of each row of logits [rows, vocab] f32 (rows row_stride elements apart, vocab
+ * <= 262144) by its own settings (device arrays of `rows`, NULL: off), where vx_lm_greedy picks
+ * the largest.  A token's weight is exp((l - lmax) / temperature), taken to 44 binary places;
+ * temperature 0 is the greedy pick.  In the order of logits (descending, ties to the lowest id)
+ *   top_k   the first k stay (k <= 0 or >= vocab: all)
+ *   top_p   of these the shortest prefix whose weight is at least top_p of theirs (>= 1: all;
+ *           at least one token)
+ *   min_p   of these the tokens of weight at least min_p times the largest
+ * and the id is the first in index order at which the sum of the staying weights exceeds u of
+ * the total, u [rows] in [0, 1).  logprob (may be NULL) receives log(weight / total).  A logit
+ * of -infinity is never drawn; +infinity leaves only its like.  A row of nothing but -infinity
+ * gives id -1 and logprob -infinity; a row that holds a NaN, or whose temperature is negative
+ * or NaN, gives id -1 and logprob NaN. */
+int vx_sample(vx_ctx* ctx, const float* logits, int64_t row_stride, int rows, int vocab, const float* u,
+              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int32_t* ids,
+              float* logprob, vx_stream stream);
+
 /* ----------------------------------------------------------------- MiniCPM-4 model */
 
 /* MiniCpmModel::new (minicpm4/model.rs:26-41) + StaticKvCache::new (minicpm4/cache.rs:21-44)

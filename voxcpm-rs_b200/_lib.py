@@ -42,6 +42,7 @@ class MiniCpm4ConfigC(C.Structure):
 
 P = C.c_void_p
 I32 = C.c_int
+I64 = C.c_int64
 F32 = C.c_float
 F64 = C.c_double
 
@@ -69,6 +70,11 @@ class VoxCpm2WeightsC(C.Structure):
                                  "fsq_out_w", "fsq_out_b")]
 
 
+class Kv4C(C.Structure):
+    _fields_ = [("k_codes", P), ("k_scales", P), ("v_codes", P), ("v_scales", P), ("weights", P), ("positions", P),
+                ("batch", C.c_int), ("n_kv_heads", C.c_int), ("capacity", C.c_int), ("head_dim", C.c_int)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "vx_version": (I32, []),
@@ -93,6 +99,12 @@ SIGNATURES = {
     "vx_mlp_swiglu": (I32, [P, P, P, P, I32, I32, I32, P, P]),
     "vx_cfg_euler": (I32, [P, P, P, I32, I32, I32, F32, F64, I32, P]),
     "vx_fsq": (I32, [P, P, P, P, P, I32, I32, I32, F32, P, I32, P, P]),
+    "vx_kv4_append": (I32, [P, P, P, P, I64, I64, I32, P, P, P, P]),
+    "vx_kv4_read": (I32, [P, P, I32, P, P, P, P, P]),
+    "vx_kv4_attend_workspace": (C.c_size_t, [P, I32, I32, I32]),
+    "vx_kv4_attend": (I32, [P, P, P, I64, I32, P, I32, F32, I32, P, I64, P, C.c_size_t, P]),
+    "vx_kv4_evict": (I32, [P, P, P, P, I32, I32, I32, I32, P, P, P, P]),
+    "vx_sample": (I32, [P, P, I64, I32, I32, P, P, P, P, P, P, P, P]),
     "vx_lm_create": (I32, [P, C.POINTER(MiniCpm4ConfigC), I32, I32, C.POINTER(P)]),
     "vx_lm_destroy": (None, [P]),
     "vx_lm_load_layer": (I32, [P, I32, P, P, P, P, P, P, P, P, P]),

@@ -126,6 +126,19 @@ inline int cuda_fail(vx_ctx* ctx, cudaError_t e, const char* where) {
 // cuBLAS), so work queued by a framework on its default stream is ordered before them.
 inline cudaStream_t pick_stream(vx_ctx*, vx_stream s) { return reinterpret_cast<cudaStream_t>(s); }
 
+// Makes a context's device the current one for a scope; the caller's comes back at its end.
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int device) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    if (prev != device) cudaSetDevice(device);
+    else prev = -1;
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
 // Ensure the context scratch has at least `bytes`; returns nullptr on failure.
 void* ctx_scratch(vx_ctx* ctx, size_t bytes);
 
@@ -162,6 +175,11 @@ const LinearWorkspace* lm_workspace(const vx_lm* lm);
 // Grow the forward() work buffers to `rows` token rows (so a later capture allocates nothing).
 int lm_prepare_rows(vx_lm* lm, size_t rows);
 cudaError_t tc_gemm_configure();
+// 4-bit KV cache and sampling (kv4*.cu, sample.cu): shared-memory limits, set once per device;
+// the checks that every kv4 entry point makes of its cache.
+cudaError_t kv4_evict_configure();
+cudaError_t sample_configure();
+int kv4_check(vx_ctx* ctx, const vx_kv4* c, const char* what);
 // AudioVAE convolutions on tcgen05 (vae_tc.cu).  launch_vae_split writes X [B, C, T] (after
 // the optional SR conditioning and snake) as the bf16 hi / lo operand xs [2][B][T][C];
 // launch_vae_tc_conv runs a pointwise conv (s = 1, A = W [Cout, Cin]) or a causal transposed
