@@ -153,7 +153,8 @@ int vx_ctx_create(int device, vx_ctx** out) {
       cudaMemset(ctx->counters, 0, 4096 * sizeof(unsigned)) != cudaSuccess ||
       cudaMalloc(&ctx->dev_err, 64) != cudaSuccess || cudaMemset(ctx->dev_err, 0, 64) != cudaSuccess ||
       gemv_configure() != cudaSuccess || tc_gemm_configure() != cudaSuccess ||
-      vae_tc_configure() != cudaSuccess || kv4_evict_configure() != cudaSuccess ||
+      vae_tc_configure() != cudaSuccess || kv4_attend_configure() != cudaSuccess ||
+      kv4_evict_configure() != cudaSuccess ||
       sample_configure() != cudaSuccess) {
     cudaGetLastError();
     delete ctx;

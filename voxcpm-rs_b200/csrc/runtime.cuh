@@ -177,6 +177,7 @@ int lm_prepare_rows(vx_lm* lm, size_t rows);
 cudaError_t tc_gemm_configure();
 // 4-bit KV cache and sampling (kv4*.cu, sample.cu): shared-memory limits, set once per device;
 // the checks that every kv4 entry point makes of its cache.
+cudaError_t kv4_attend_configure();
 cudaError_t kv4_evict_configure();
 cudaError_t sample_configure();
 int kv4_check(vx_ctx* ctx, const vx_kv4* c, const char* what);
