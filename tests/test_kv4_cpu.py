@@ -57,20 +57,21 @@ def test_buffers_of_another_device_are_refused():
 
 @pytest.fixture
 def host_cache(monkeypatch):
-    """A cache over host tensors: the classes' own checks, with the device check aimed at the CPU."""
+    """A cache over host tensors (whose device index is -1): the classes' own checks alone."""
     import torch
     from voxcpm_rs_b200 import kv4
+
+    class Lib:
+        def __getattr__(self, n):
+            return (lambda *a: 0) if n.endswith("workspace") else (lambda *a: pytest.fail(n + " was called"))
 
     class Torch:
         def __getattr__(self, n):
             return (lambda *a: torch.device("cpu")) if n == "device" else getattr(torch, n)
 
-    monkeypatch.setattr(kv4, "_torch", lambda: Torch())
-    class Lib:
-        def __getattr__(self, n):
-            return (lambda *a: 0) if n.endswith("workspace") else (lambda *a: pytest.fail(n + " was called"))
-
     monkeypatch.setattr(kv4, "lib", Lib)
+    monkeypatch.setattr(kv4, "_torch", Torch)
+    monkeypatch.setattr(_Ctx, "device", -1)
     w, p = torch.zeros(1, 2, 64), torch.zeros(1, 2, 64, dtype=torch.int64)
     return kv4.Kv4Cache.from_buffers(_Ctx(), *_bufs(), weights=w, positions=p)
 

@@ -1,11 +1,16 @@
 // Eviction from the 4-bit KV cache by accumulated attention weight (vx_kv4_evict).
 //
 // One cluster of C thread blocks per (sequence, KV head).  A row's rank is its weight as an
-// ordered 32-bit key (protected rows: the largest key); four 8-bit radix passes over the keys
-// find the key T of the keep-th largest row and how many rows of key T stay (those of the lowest
+// ordered 32-bit key (protected rows: the largest key); 8-bit radix passes over the keys find
+// the key T of the keep-th largest row and how many rows of key T stay (those of the lowest
 // slots).  Attention does not depend on the order of rows, so nothing is shifted: the i-th slot
 // below `keep` that became free takes the i-th kept row behind it.  Sources (slots >= keep) and
 // destinations (slots < keep) are disjoint, so the moves need no order among them.
+//
+// What bounds it is latency: a pass is a shared-memory histogram, a cluster barrier and a scan.
+// So the keys are read once and stay in registers (slot order is warp, item, lane: a scan over
+// all slots is one ballot per item and one sum over warps), every pass has one cluster barrier,
+// and the passes end as soon as a digit's rows all stay.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -17,9 +22,11 @@ namespace cg = cooperative_groups;
 namespace vx {
 namespace {
 
-constexpr int EV_THREADS = 1024;
+constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
 constexpr int EV_MAX_CLUSTER = 8;
-constexpr int EV_MAX_LEN = 131072;
+constexpr int EV_MAX_ITEMS = 32;  // keys of a thread
+constexpr int EV_MAX_LEN = EV_THREADS * EV_MAX_CLUSTER * EV_MAX_ITEMS;  // 131072
+static_assert(EV_MAX_LEN == 131072, "the length that the header names");
 
 struct EvictArgs {
   uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
@@ -29,7 +36,7 @@ struct EvictArgs {
   int64_t* positions_out;
   const int *lens, *seen;
   int* lens_out;
-  int B, nkv, d, cap, max_len, keep, sink, recent, seg_max;
+  int B, nkv, d, cap, max_len, keep, sink, recent;
   int* err;
 };
 
@@ -40,191 +47,260 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+struct EvictShared {
+  uint32_t hist[3][256], tot[256];
+  uint32_t warp_n[2][EV_WARPS];
+  uint32_t eq, holes, movers;  // of this block; read by the cluster
+};
+
+// Sum over the warps before this one and over all, of a value that each warp has put in n[].
+__device__ __forceinline__ uint32_t warps_before(const uint32_t* n, int warp, uint32_t* all) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t v = lane < EV_WARPS ? n[lane] : 0;
+  *all = __reduce_add_sync(0xffffffffu, v);
+  return __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+}
+
+template <int ITEMS>
 __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a) {
-  extern __shared__ __align__(16) uint32_t dyn[];  // keys [seg_max], then slot lists
-  __shared__ uint32_t hist[2][256], tot[256];
-  __shared__ uint32_t warp_n[32], sh[8];
+  extern __shared__ __align__(16) uint32_t list[];  // free slots from the front, movers from the back
+  __shared__ EvictShared s;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int unit = blockIdx.x / C, b = unit / a.nkv, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = a.lens[b];
   const size_t row0 = (size_t)unit * a.cap;
+  const bool first = unit % a.nkv == 0 && rank == 0 && tid == 0;
   if (n < 0 || n > a.max_len) {  // the same for every block of the cluster
-    if (unit % a.nkv == 0 && rank == 0 && tid == 0) {
+    if (first) {
       record_error(a.err, VX_DEVICE_ERR_BOUNDS);
       a.lens_out[b] = n;
     }
     return;
   }
-  if (unit % a.nkv == 0 && rank == 0 && tid == 0) a.lens_out[b] = min(n, a.keep);
+  if (first) a.lens_out[b] = min(n, a.keep);
   if (a.keep == 0) return;  // every row goes
-  if (n <= a.keep) {  // nothing to let go of
+  if (n <= a.keep) {        // every row stays
     for (int j = rank * EV_THREADS + tid; j < n; j += C * EV_THREADS) {
       if (a.weights_out != a.weights) a.weights_out[row0 + j] = a.weights[row0 + j];
       if (a.positions_out != a.positions) a.positions_out[row0 + j] = a.positions[row0 + j];
     }
     return;
   }
-  const int seg = (n + C - 1) / C, lo = min(n, rank * seg), hi = min(n, lo + seg), cnt = hi - lo;
-  uint32_t* keys = dyn;
-  uint32_t* list = dyn + a.seg_max;  // this block's free slots from the front, its movers from the back
+  const int base = (rank * EV_WARPS + warp) * 32 * ITEMS + lane;  // slot of item i: base + 32 i
   const int64_t since = (int64_t)a.seen[b] - a.recent;
-  for (int j = tid; j < cnt; j += EV_THREADS) {
-    const int64_t pos = a.positions[row0 + lo + j];
-    keys[j] = (pos < a.sink || pos >= since) ? 0xffffffffu : weight_key(a.weights[row0 + lo + j]);
+  uint32_t key[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int j = base + 32 * i;
+    key[i] = 0;
+    if (j < n) {
+      const int64_t pos = a.positions[row0 + j];
+      const float w = a.weights[row0 + j];
+      key[i] = (pos < a.sink || pos >= since) ? 0xffffffffu : weight_key(w);
+    }
   }
-  uint32_t prefix = 0, left = (uint32_t)a.keep;  // rows still to be found among the keys of this prefix
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    uint32_t* h = hist[pass & 1];
-    if (tid < 256) h[tid] = 0;
-    __syncthreads();
-    for (int j = tid; j < cnt; j += EV_THREADS) {
-      const uint32_t k = keys[j];
-      if (pass == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&h[(k >> shift) & 255], 1u);
+  if (tid < 256) s.hist[0][tid] = 0;
+  __syncthreads();
+  uint32_t T = 0, left = (uint32_t)a.keep;  // rows still to be found among the keys that begin like T
+  bool all_stay = false;                    // every key of T's digits so far stays
+  for (int shift = 24, p = 0; shift >= 0 && !all_stay; shift -= 8, ++p) {
+    uint32_t* h = s.hist[p % 3];
+    if (tid < 256) s.hist[(p + 1) % 3][tid] = 0;  // last read two passes ago
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const bool mine = base + 32 * i < n && (shift == 24 || ((key[i] ^ T) >> (shift + 8)) == 0);
+      // lanes of the same digit add once: weights share their leading digits
+      const uint32_t d = mine ? (key[i] >> shift) & 255 : 256;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (mine && lane == __ffs(same) - 1) atomicAdd(&h[d], (uint32_t)__popc(same));
     }
     cl.sync();
     if (tid < 256) {
       uint32_t t = 0;
       for (int r = 0; r < C; ++r) t += cl.map_shared_rank(h, r)[tid];
-      tot[tid] = t;
+      s.tot[tid] = t;
     }
     __syncthreads();
-    if (warp == 0) {  // the digit at which the count from above reaches `left`
-      uint32_t v[8], s = 0;
-      for (int e = 0; e < 8; ++e) s += v[e] = tot[255 - (lane * 8 + e)];
-      uint32_t incl = s;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
-      }
-      uint32_t above = incl - s;
-      if (above < left && incl >= left) {
-        int e = 0;
-        while (above + v[e] < left) above += v[e++];
-        sh[0] = prefix | ((uint32_t)(255 - (lane * 8 + e)) << shift);
-        sh[1] = left - above;
-      }
+    // every warp finds the digit at which the count from above reaches `left`
+    uint32_t v[8], sum = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += v[e] = s.tot[255 - (lane * 8 + e)];
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
     }
-    __syncthreads();
-    prefix = sh[0];
-    left = sh[1];
+    const uint32_t hit = __ballot_sync(0xffffffffu, incl >= left);
+    const int at = __ffs(hit) - 1;
+    uint32_t above = incl - sum, digit = 255 - lane * 8, cnt = v[0];
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (above + v[e] < left && digit == (uint32_t)(255 - lane * 8 - e)) {
+        above += v[e];
+        --digit;
+        cnt = v[e + 1];
+      }
+    above = __shfl_sync(0xffffffffu, above, at);
+    digit = __shfl_sync(0xffffffffu, digit, at);
+    cnt = __shfl_sync(0xffffffffu, cnt, at);
+    left -= above;
+    T |= digit << shift;
+    all_stay = cnt == left;
+    __syncthreads();  // tot is read
   }
-  const uint32_t T = prefix, ties = left;  // `ties` rows of key T stay, in slot order
 
-  // how many rows of key T lie in the blocks before this one
-  uint32_t c = 0;
-  for (int j = tid; j < cnt; j += EV_THREADS) c += keys[j] == T;
-  c = __reduce_add_sync(0xffffffffu, c);
-  if (lane == 0) warp_n[warp] = c;
+  // rows of key T that stay: all of them, or the first `left` in slot order
+  uint32_t eq_before = 0;
+  if (!all_stay) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) c += __popc(__ballot_sync(0xffffffffu, base + 32 * i < n && key[i] == T));
+    if (lane == 0) s.warp_n[0][warp] = c;
+    __syncthreads();
+    uint32_t all;
+    eq_before = warps_before(s.warp_n[0], warp, &all);
+    if (tid == 0) s.eq = all;
+    cl.sync();
+    const uint32_t e = lane < rank ? *cl.map_shared_rank(&s.eq, lane) : 0;
+    eq_before += __reduce_add_sync(0xffffffffu, e);
+  }
+  const uint32_t below = (1u << lane) - 1;
+  uint32_t stays = 0, holes = 0, movers = 0;  // bit i: item i; counts of this warp
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int j = base + 32 * i;
+    bool keep = j < n && key[i] >= T;
+    if (!all_stay) {
+      const bool eq = j < n && key[i] == T;
+      const uint32_t m = __ballot_sync(0xffffffffu, eq);
+      if (eq) keep = eq_before + __popc(m & below) < left;
+      eq_before += __popc(m);
+    }
+    stays |= (uint32_t)keep << i;
+    holes += __popc(__ballot_sync(0xffffffffu, j < n && j < a.keep && !keep));
+    movers += __popc(__ballot_sync(0xffffffffu, j >= a.keep && keep));
+  }
+  if (lane == 0) s.warp_n[1][warp] = holes | movers << 16;  // at most 16384 each in a block
   __syncthreads();
-  if (warp == 0) {
-    c = __reduce_add_sync(0xffffffffu, warp_n[lane]);
-    if (lane == 0) sh[2] = c;
-  }
-  cl.sync();
-  uint32_t eq_base = 0;
-  for (int r = 0; r < rank; ++r) eq_base += *cl.map_shared_rank(&sh[2], r);
-
-  // free slots and movers of this block, in slot order
-  uint32_t holes = 0, movers = 0;
-  for (int j0 = 0; j0 < cnt; j0 += EV_THREADS) {
-    const int j = j0 + tid, slot = lo + j;
-    const bool in = j < cnt;
-    const uint32_t k = in ? keys[j] : 0;
-    const uint32_t eq = __ballot_sync(0xffffffffu, in && k == T);
-    __syncthreads();
-    if (lane == 0) warp_n[warp] = __popc(eq);
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) before += warp_n[w];
-      all += warp_n[w];
-    }
-    const uint32_t tr = eq_base + before + __popc(eq & ((1u << lane) - 1));
-    eq_base += all;
-    const bool stays = in && (k > T || (k == T && tr < ties));
-    const bool hole = in && slot < a.keep && !stays, mover = stays && slot >= a.keep;
-    const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
-    __syncthreads();
-    if (lane == 0) warp_n[warp] = __popc(hb) | (__popc(mb) << 16);
-    __syncthreads();
-    before = all = 0;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) before += warp_n[w];
-      all += warp_n[w];
-    }
-    const uint32_t below = (1u << lane) - 1;
-    if (hole) list[holes + (before & 0xffff) + __popc(hb & below)] = slot;
-    if (mover) list[a.seg_max - 1 - (movers + (before >> 16) + __popc(mb & below))] = slot;
-    holes += all & 0xffff;
-    movers += all >> 16;
-    if (stays && slot < a.keep) {
-      if (a.weights_out != a.weights) a.weights_out[row0 + slot] = a.weights[row0 + slot];
-      if (a.positions_out != a.positions) a.positions_out[row0 + slot] = a.positions[row0 + slot];
-    }
-  }
+  uint32_t all;
+  const uint32_t before = warps_before(s.warp_n[1], warp, &all);
   if (tid == 0) {
-    sh[3] = holes;
-    sh[4] = movers;
+    s.holes = all & 0xffff;
+    s.movers = all >> 16;
   }
-  cl.sync();
-  uint32_t m0 = 0, hole0[EV_MAX_CLUSTER + 1];
-  hole0[0] = 0;
+  uint32_t hb = before & 0xffff, mb = before >> 16;
+  constexpr int kLast = EV_THREADS * ITEMS - 1;
 #pragma unroll
-  for (int r = 0; r < EV_MAX_CLUSTER; ++r) {
-    hole0[r + 1] = hole0[r];
-    if (r < C) {
-      if (r < rank) m0 += *cl.map_shared_rank(&sh[4], r);
-      hole0[r + 1] += *cl.map_shared_rank(&sh[3], r);
+  for (int i = 0; i < ITEMS; ++i) {
+    const int j = base + 32 * i;
+    const bool keep = stays >> i & 1, hole = j < n && j < a.keep && !keep, mover = j >= a.keep && keep;
+    const uint32_t hm = __ballot_sync(0xffffffffu, hole), mm = __ballot_sync(0xffffffffu, mover);
+    if (hole) list[hb + __popc(hm & below)] = j;
+    if (mover) list[kLast - (mb + __popc(mm & below))] = j;
+    hb += __popc(hm);
+    mb += __popc(mm);
+    if (keep && j < a.keep) {
+      if (a.weights_out != a.weights) a.weights_out[row0 + j] = a.weights[row0 + j];
+      if (a.positions_out != a.positions) a.positions_out[row0 + j] = a.positions[row0 + j];
     }
   }
-  // 16 lanes move a row
-  const int cb = a.d / 32, sb = a.d / 16;  // 16-byte pieces of the codes, bytes of the scales
-  const int l16 = tid & 15;
-  for (uint32_t i = tid >> 4; i < movers; i += EV_THREADS / 16) {
-    const size_t src = row0 + list[a.seg_max - 1 - i];
-    const uint32_t g = m0 + i;
-    int owner = 0;
-    uint32_t first = 0;
+  cl.sync();
+  // lane r: free slots and movers of the blocks before block r
+  const uint32_t h_r = lane < C ? *cl.map_shared_rank(&s.holes, lane) : 0;
+  const uint32_t m0 = __reduce_add_sync(0xffffffffu, lane < rank ? *cl.map_shared_rank(&s.movers, lane) : 0);
+  uint32_t hole0 = h_r;
 #pragma unroll
-    for (int r = 1; r < EV_MAX_CLUSTER; ++r)
-      if (g >= hole0[r]) {
-        owner = r;
-        first = hole0[r];
+  for (int o = 1; o < EV_MAX_CLUSTER; o <<= 1) {
+    const uint32_t t = __shfl_up_sync(0xffffffffu, hole0, o);
+    if (lane >= o) hole0 += t;
+  }
+  hole0 -= h_r;
+  const uint32_t mine = all >> 16;
+  // 16 lanes move a row, four rows at a time to have their loads in flight together
+  const int l16 = tid & 15, cb = a.d / 32, sb = a.d / 64;  // 16-byte pieces of a row's codes, words of its scales
+  const uint8_t* src_base;
+  uint8_t* dst_base;
+  int row_bytes, kind;  // 0: 16 bytes, 1: 4 bytes, 2: 8 bytes
+  if (l16 < 2 * cb) {
+    kind = 0, row_bytes = a.d / 2;
+    dst_base = (l16 < cb ? a.k_codes : a.v_codes) + (l16 % cb) * 16;
+    src_base = dst_base;
+  } else if (l16 < 2 * cb + 2 * sb) {
+    const int i = l16 - 2 * cb;
+    kind = 1, row_bytes = a.d / 16;
+    dst_base = (i < sb ? a.k_scales : a.v_scales) + (i % sb) * 4;
+    src_base = dst_base;
+  } else if (l16 == 14) {
+    kind = 1, row_bytes = 4;
+    src_base = reinterpret_cast<const uint8_t*>(a.weights);
+    dst_base = reinterpret_cast<uint8_t*>(a.weights_out);
+  } else if (l16 == 15) {
+    kind = 2, row_bytes = 8;
+    src_base = reinterpret_cast<const uint8_t*>(a.positions);
+    dst_base = reinterpret_cast<uint8_t*>(a.positions_out);
+  } else {
+    kind = 3, row_bytes = 0, src_base = nullptr, dst_base = nullptr;
+  }
+  src_base += row0 * row_bytes;
+  dst_base += row0 * row_bytes;
+  constexpr int kRows = EV_THREADS / 16;
+  for (uint32_t i0 = tid >> 4; i0 < (mine + kRows - 1) / kRows * kRows; i0 += 4 * kRows) {
+    uint4 x[4];
+    uint32_t dst[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t i = i0 + u * kRows, g = m0 + i;
+      // block that holds the g-th free slot: the last one whose first is not above g
+      uint32_t owner = 0, start = 0;
+#pragma unroll
+      for (int r = 1; r < EV_MAX_CLUSTER; ++r) {
+        const uint32_t f = __shfl_sync(0xffffffffu, hole0, r);
+        if (r < C && g >= f) owner = r, start = f;
       }
-    const size_t dst = row0 + cl.map_shared_rank(list, owner)[g - first];
-    if (l16 < cb)
-      reinterpret_cast<uint4*>(a.k_codes + dst * (a.d / 2))[l16] =
-          reinterpret_cast<const uint4*>(a.k_codes + src * (a.d / 2))[l16];
-    else if (l16 < 2 * cb)
-      reinterpret_cast<uint4*>(a.v_codes + dst * (a.d / 2))[l16 - cb] =
-          reinterpret_cast<const uint4*>(a.v_codes + src * (a.d / 2))[l16 - cb];
-    else if (l16 < 2 * cb + sb / 4)
-      reinterpret_cast<uint32_t*>(a.k_scales + dst * sb)[l16 - 2 * cb] =
-          reinterpret_cast<const uint32_t*>(a.k_scales + src * sb)[l16 - 2 * cb];
-    else if (l16 < 2 * cb + sb / 2)
-      reinterpret_cast<uint32_t*>(a.v_scales + dst * sb)[l16 - 2 * cb - sb / 4] =
-          reinterpret_cast<const uint32_t*>(a.v_scales + src * sb)[l16 - 2 * cb - sb / 4];
-    else if (l16 == 14)
-      a.weights_out[dst] = a.weights[src];
-    else if (l16 == 15)
-      a.positions_out[dst] = a.positions[src];
+      dst[u] = 0xffffffffu;
+      if (i < mine) {
+        dst[u] = cl.map_shared_rank(list, owner)[g - start];
+        const uint8_t* p = src_base + (size_t)list[kLast - i] * row_bytes;
+        if (kind == 0) x[u] = *reinterpret_cast<const uint4*>(p);
+        if (kind == 1) x[u].x = *reinterpret_cast<const uint32_t*>(p);
+        if (kind == 2) *reinterpret_cast<uint2*>(&x[u]) = *reinterpret_cast<const uint2*>(p);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (dst[u] != 0xffffffffu) {
+        uint8_t* p = dst_base + (size_t)dst[u] * row_bytes;
+        if (kind == 0) *reinterpret_cast<uint4*>(p) = x[u];
+        if (kind == 1) *reinterpret_cast<uint32_t*>(p) = x[u].x;
+        if (kind == 2) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(&x[u]);
+      }
   }
   cl.sync();  // the lists are read by the other blocks
 }
 
-int cluster_of(int max_len) {
-  int c = 1;
-  while (c < EV_MAX_CLUSTER && max_len > 4096 * c) c *= 2;
-  return c;
+// Blocks of a cluster and keys of a thread: as many blocks as keep about two on each SM, as few
+// keys as hold the longest sequence.
+void evict_shape(int units, int max_len, int* C, int* items) {
+  *C = 1;
+  while (*C < EV_MAX_CLUSTER && max_len > EV_THREADS * 2 * *C && units * *C * 2 <= 296) *C *= 2;
+  while (max_len > EV_THREADS * EV_MAX_ITEMS * *C) *C *= 2;
+  *items = 2;
+  while (max_len > EV_THREADS * *items * *C) *items *= 2;
+}
+
+template <int ITEMS>
+cudaError_t evict_launch(cudaLaunchConfig_t& cfg, const EvictArgs& a) {
+  cfg.dynamicSmemBytes = (size_t)EV_THREADS * ITEMS * 4;
+  return cudaLaunchKernelEx(&cfg, kv4_evict_kernel<ITEMS>, a);
 }
 
 }  // namespace
 
 cudaError_t kv4_evict_configure() {
-  return cudaFuncSetAttribute(kv4_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              EV_MAX_LEN / EV_MAX_CLUSTER * 8);
+  return cudaFuncSetAttribute(kv4_evict_kernel<EV_MAX_ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              EV_THREADS * EV_MAX_ITEMS * 4);
 }
 
 }  // namespace vx
@@ -246,16 +322,14 @@ extern "C" int vx_kv4_evict(vx_ctx* ctx, const vx_kv4* c, const int32_t* lens, c
   if (keep < 0 || sink < 0 || recent < 0 || (long long)sink + recent > keep)
     return fail(ctx, VX_ERR_SHAPE, "kv4_evict: sink %d + recent %d must fit in keep %d", sink, recent, keep);
   DeviceGuard guard(ctx->device);
-  const int C = cluster_of(max_len);
-  const int seg = std::max(1, (max_len + C - 1) / C);
-  const size_t smem = (size_t)seg * 2 * 4;
   EvictArgs a = {c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->weights, c->positions, weights_out,
                  positions_out, lens, seen, lens_out, c->batch, c->n_kv_heads, c->head_dim, c->capacity, max_len, keep,
-                 sink, recent, seg, ctx->dev_err};
+                 sink, recent, ctx->dev_err};
+  int C, items;
+  evict_shape(c->batch * c->n_kv_heads, max_len, &C, &items);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(c->batch * c->n_kv_heads * C);
   cfg.blockDim = dim3(EV_THREADS);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = pick_stream(ctx, stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -265,6 +339,10 @@ extern "C" int vx_kv4_evict(vx_ctx* ctx, const vx_kv4* c, const int32_t* lens, c
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  VX_CUDA(ctx, cudaLaunchKernelEx(&cfg, kv4_evict_kernel, a));
+  VX_CUDA(ctx, items == 2    ? evict_launch<2>(cfg, a)
+               : items == 4  ? evict_launch<4>(cfg, a)
+               : items == 8  ? evict_launch<8>(cfg, a)
+               : items == 16 ? evict_launch<16>(cfg, a)
+                             : evict_launch<32>(cfg, a));
   return VX_OK;
 }

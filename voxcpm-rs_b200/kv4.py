@@ -8,24 +8,23 @@ allocate their outputs and workspace there, so they can be captured into a CUDA 
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 from . import _lib
 from ._lib import VX_ERR_ARG, VX_ERR_SHAPE, VxError, check, lib
-from .minicpm4 import Context, _torch
+from .minicpm4 import Context, _torch, raw_stream
 
 
 def _refuse(code, msg):
     raise VxError(code, msg)
 
 
-def _need(t, what, dtype, shape, device):
-    """`t` is a contiguous tensor of this type, shape and device, else the call is refused."""
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
-        _refuse(VX_ERR_ARG, f"{what}: a contiguous {dtype} tensor on {device} is needed, "
+def _need(t, what, dtype, shape, index):
+    """`t` is a contiguous tensor of this type and shape on cuda:`index`, else the call is refused."""
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+        _refuse(VX_ERR_ARG, f"{what}: a contiguous {dtype} tensor on cuda:{index} is needed, "
                             f"got {t.dtype} on {t.device}{'' if t.is_contiguous() else ', strided'}")
-    if tuple(t.shape) != shape:
-        _refuse(VX_ERR_SHAPE, f"{what}: shape {shape} is needed, got {tuple(t.shape)}")
+    if t.shape != shape:
+        _refuse(VX_ERR_SHAPE, f"{what}: shape {tuple(shape)} is needed, got {tuple(t.shape)}")
 
 
 class Kv4Cache:
@@ -59,65 +58,65 @@ class Kv4Cache:
         if k_codes.dim() != 4:
             _refuse(VX_ERR_SHAPE, "k_codes: [batch, n_kv_heads, capacity, head_dim / 2] is needed")
         b, nkv, cap, half = k_codes.shape
-        dev = torch.device("cuda", ctx.device)
         for t, what in ((k_codes, "k_codes"), (v_codes, "v_codes")):
-            _need(t, what, torch.uint8, (b, nkv, cap, half), dev)
+            _need(t, what, torch.uint8, (b, nkv, cap, half), ctx.device)
         for t, what in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-            _need(t, what, torch.float8_e4m3fn, (b, nkv, cap, half // 8), dev)
+            _need(t, what, torch.float8_e4m3fn, (b, nkv, cap, half // 8), ctx.device)
         for t, what, dt in ((weights, "weights", torch.float32), (positions, "positions", torch.int64)):
             if t is not None:
-                _need(t, what, dt, (b, nkv, cap), dev)
-        self.ctx, self.device = ctx, dev
+                _need(t, what, dt, (b, nkv, cap), ctx.device)
+        self.ctx, self.device, self._index = ctx, torch.device("cuda", ctx.device), ctx.device
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.weights, self.positions = weights, positions
         self.batch, self.n_kv_heads, self.capacity, self.head_dim = b, nkv, cap, 2 * half
         p = [None if t is None else t.data_ptr() for t in (k_codes, k_scales, v_codes, v_scales, weights, positions)]
         self._c = _lib.Kv4C(*p, b, nkv, cap, 2 * half)
         self._ref = C.addressof(self._c)
+        self._lens_shape = torch.Size((b,))
         self._plans = {}
 
     def _ints(self, t, what):
         if t is None:
             return None
-        torch = _torch()
-        _need(t, what, torch.int32, (self.batch,), self.device)
+        _need(t, what, _torch().int32, self._lens_shape, self._index)
         return t.data_ptr()
 
-    def _stream(self):
-        return _torch().cuda.current_stream(self.device).cuda_stream
+    def _run(self, fn, *args):
+        """One call of the library on the current stream of the cache's device."""
+        rc = fn(self.ctx.h, self._ref, *args, raw_stream(self._index))
+        if rc:
+            check(rc, self.ctx.h)
 
     def append(self, k, v, start, counts=None, first_position=None):
         """Quantise the rows of new tokens into the cache: ``k``, ``v`` f32 ``[B, S, nkv, d]``, the
         last two dims dense (views into a fused projection will do), token ``i < counts[b]`` into
         slot ``start[b] + i``.  Their weights become 0 and their positions
         ``first_position[b] + i`` (the slot without it)."""
-        torch = _torch()
+        f32 = _torch().float32
         s = k.shape[1] if k.dim() == 4 else -1
         for t, what in ((k, "k"), (v, "v")):
-            if tuple(t.shape) != (self.batch, s, self.n_kv_heads, self.head_dim):
+            if t.shape != (self.batch, s, self.n_kv_heads, self.head_dim):
                 _refuse(VX_ERR_SHAPE, f"{what}: [{self.batch}, S, {self.n_kv_heads}, {self.head_dim}] is needed, "
                                       f"got {tuple(t.shape)}")
-            if t.dtype != torch.float32 or t.device != self.device:
+            if t.dtype is not f32 or t.get_device() != self._index:
                 _refuse(VX_ERR_ARG, f"{what}: f32 on {self.device} is needed, got {t.dtype} on {t.device}")
         if s == 0:
             return
-        dense = all(t.stride(3) == 1 and (t.stride(2) == self.head_dim or self.n_kv_heads == 1) for t in (k, v))
-        if not dense or k.stride()[:2] != v.stride()[:2]:
+        st = k.stride()
+        if st != v.stride() or st[3] != 1 or (st[2] != self.head_dim and self.n_kv_heads != 1):
             _refuse(VX_ERR_ARG, "k and v: dense heads and the same strides are needed")
-        check(lib().vx_kv4_append(self.ctx.h, self._ref, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), s,
-                                  self._ints(start, "start"), self._ints(counts, "counts"),
-                                  self._ints(first_position, "first_position"), self._stream()), self.ctx.h)
+        self._run(lib().vx_kv4_append, k.data_ptr(), v.data_ptr(), st[0], st[1], s, self._ints(start, "start"),
+                  self._ints(counts, "counts"), self._ints(first_position, "first_position"))
 
     def read(self, n, start=None, counts=None):
         """The values of rows ``start[b] + i`` (``i < counts[b] <= n``; zeros behind them) as
         ``k, v`` f32 ``[B, nkv, n, d]``."""
         torch = _torch()
-        k = torch.empty(self.batch, self.n_kv_heads, n, self.head_dim, device=self.device)
-        v = torch.empty_like(k)
+        shape = (self.batch, self.n_kv_heads, n, self.head_dim)
+        k, v = torch.empty(shape, device=self.device), torch.empty(shape, device=self.device)
         if n:
-            check(lib().vx_kv4_read(self.ctx.h, self._ref, n, self._ints(start, "start"),
-                                    self._ints(counts, "counts"), k.data_ptr(), v.data_ptr(), self._stream()),
-                  self.ctx.h)
+            self._run(lib().vx_kv4_read, n, self._ints(start, "start"), self._ints(counts, "counts"), k.data_ptr(),
+                      v.data_ptr())
         return k, v
 
     def attend(self, q, lens, max_len=None, track=False, scale=None):
@@ -126,24 +125,22 @@ class Kv4Cache:
         work is split for that length).  Returns ``[B, nh * d]``.  With ``track`` the rows'
         ``weights`` grow by the probabilities that they received."""
         torch = _torch()
-        if q.dtype != torch.float32 or q.device != self.device:
+        if q.dtype is not torch.float32 or q.get_device() != self._index:
             _refuse(VX_ERR_ARG, f"q: f32 on {self.device} is needed, got {q.dtype} on {q.device}")
         if q.dim() != 2 or q.shape[0] != self.batch or q.shape[1] % self.head_dim or q.stride(1) != 1:
             _refuse(VX_ERR_SHAPE, f"q: dense rows [{self.batch}, nh * {self.head_dim}] are needed, got {tuple(q.shape)}")
-        nh = q.shape[1] // self.head_dim
+        width = q.shape[1]
+        nh = width // self.head_dim
         n = self.capacity if max_len is None else max_len
-        L = lib()
         key = (nh, n, bool(track))
         need = self._plans.get(key)
         if need is None:
-            need = self._plans[key] = L.vx_kv4_attend_workspace(self._ref, *key)
-        out = torch.empty(self.batch, nh * self.head_dim, device=self.device)
+            need = self._plans[key] = lib().vx_kv4_attend_workspace(self._ref, *key)
+        out = torch.empty((self.batch, width), device=self.device)
         ws = torch.empty(need, device=self.device, dtype=torch.uint8) if need else None
-        check(L.vx_kv4_attend(self.ctx.h, self._ref, q.data_ptr(), q.stride(0) if self.batch > 1 else q.shape[1], nh,
-                              self._ints(lens, "lens"), n,
-                              1.0 / math.sqrt(self.head_dim) if scale is None else scale, track,
-                              out.data_ptr(), out.shape[1], None if ws is None else ws.data_ptr(), need,
-                              self._stream()), self.ctx.h)
+        self._run(lib().vx_kv4_attend, q.data_ptr(), q.stride(0) if self.batch > 1 else width, nh,
+                  self._ints(lens, "lens"), n, self.head_dim ** -0.5 if scale is None else scale, track,
+                  out.data_ptr(), width, None if ws is None else ws.data_ptr(), need)
         return out
 
     def evict(self, lens, seen, keep, sink=0, recent=0, max_len=None, weights_out=None, positions_out=None):
@@ -157,10 +154,10 @@ class Kv4Cache:
             _refuse(VX_ERR_ARG, "evict: the cache keeps no weights and positions")
         wo = self.weights if weights_out is None else weights_out
         po = self.positions if positions_out is None else positions_out
-        _need(wo, "weights_out", torch.float32, tuple(self.weights.shape), self.device)
-        _need(po, "positions_out", torch.int64, tuple(self.positions.shape), self.device)
-        out = torch.empty(self.batch, device=self.device, dtype=torch.int32)
-        check(lib().vx_kv4_evict(self.ctx.h, self._ref, self._ints(lens, "lens"), self._ints(seen, "seen"),
-                                 self.capacity if max_len is None else max_len, keep, sink, recent, wo.data_ptr(),
-                                 po.data_ptr(), out.data_ptr(), self._stream()), self.ctx.h)
+        _need(wo, "weights_out", torch.float32, self.weights.shape, self._index)
+        _need(po, "positions_out", torch.int64, self.positions.shape, self._index)
+        out = torch.empty(self._lens_shape, device=self.device, dtype=torch.int32)
+        self._run(lib().vx_kv4_evict, self._ints(lens, "lens"), self._ints(seen, "seen"),
+                  self.capacity if max_len is None else max_len, keep, sink, recent, wo.data_ptr(), po.data_ptr(),
+                  out.data_ptr())
         return out

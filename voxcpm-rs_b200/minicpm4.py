@@ -70,6 +70,12 @@ class Context:
             pass
 
 
+def raw_stream(index):
+    """The ``cudaStream_t`` of torch's current stream of a device, without the Stream object that
+    ``torch.cuda.current_stream`` builds (0.1 instead of 2 us of a call)."""
+    return _torch()._C._cuda_getCurrentRawStream(index)
+
+
 def _stream_of(t):
     torch = _torch()
     return torch.cuda.current_stream(t.device).cuda_stream
