@@ -27,17 +27,18 @@ def test_null_arguments_are_refused():
 
 
 def test_attend_workspace():
-    """0 for arguments that a call refuses; it grows with the length, and a tracking call's holds a
-    score of 8 query heads for each row."""
+    """0 for arguments that a call refuses and for short sequences; else it grows with the length,
+    and a tracking call's holds a score of 8 query heads for each row."""
     from voxcpm_rs_b200 import _lib
     f = _lib.lib().vx_kv4_attend_workspace
     c = _lib.Kv4C(None, None, None, None, None, None, 2, 2, 131072, 128)
     ref = C.addressof(c)
     assert f(None, 8, 10, 0) == 0 and f(ref, 0, 10, 0) == 0 and f(ref, 3, 10, 0) == 0 and f(ref, 16, -1, 0) == 0
-    assert f(ref, 16, 1, 0) == 0
-    assert f(ref, 16, 131072, 0) > f(ref, 16, 4096, 0) > 0
-    for n in (1, 33, 5000):
+    assert [f(ref, 16, n, t) for n in (0, 1, 500, 4096) for t in (0, 1)] == [0] * 8
+    assert f(ref, 16, 131072, 0) > f(ref, 16, 8192, 0) > 0
+    for n in (5000, 131072):
         assert f(ref, 16, n, 1) >= f(ref, 16, n, 0) + 2 * 2 * n * 8 * 4
+    assert f(ref, 32, 100, 1) >= 2 * 2 * 2 * 100 * 8 * 4  # 16 query heads share a KV head: two blocks of them
 
 
 def _bufs(b=1, nkv=2, cap=64, d=64):

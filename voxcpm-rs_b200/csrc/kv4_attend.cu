@@ -3,14 +3,19 @@
 // `track` the running weight of a row += the sum of p_j over the query heads that share it.
 //
 // kv4_split_kernel: grid (splits, B * nkv * head blocks of up to 8 query heads); a split covers
-// a run of positions and leaves (m, l, o) of its heads, or the result where there is one split.
-// kv4_finish_kernel: merges the splits, and turns the scores that a tracking call left in the
-// workspace into weights once the maxima and sums over all splits are known.
+// a run of positions.  Up to 8 splits are one thread-block cluster, which joins their (m, l, o)
+// through distributed shared memory and has its scores there for `track`: one launch, no
+// workspace.  More splits leave them in the workspace, and kv4_finish_kernel joins them and turns
+// the scores that a tracking call left there into weights.
+#include <cooperative_groups.h>
+
 #include <cfloat>
 
 #include "common.cuh"
 #include "kv4.cuh"
 #include "runtime.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace vx {
 namespace {
@@ -43,27 +48,40 @@ __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
 // Each warp walks its own tiles of 32 positions, with no barrier between the warps of a block
 // until the end.  Both products run on m16n8k16 f16 tensor instructions with f32 sums, and are
 // exact in what they multiply: a cached value has at most 6 significant bits and is made as f16
-// from its code and scale; a query and a probability are split into two f16 terms (22 bits),
-// and the 16 rows of an instruction are the first terms of 8 query heads and their second terms,
-// whose sums are added afterwards.
-//   S = Q K^T: the contracted index may be taken in any order, so thread (g, t) of the B operand
-//     reads D / 4 dims of row g in one piece (16 or 8 bytes): k-step s takes its bytes 2s, 2s + 1.
-//   O = P V: n-tile j's column g is dim g D/8 + j, so thread (g, t) reads one piece of 8 or 4 bytes
-//     of each of its 4 positions; the pairs along positions that the operand needs are made by
+// from its code and scale; a query and a probability are split into two f16 terms (22 bits).
+//   S = Q K^T: the 16 rows are the first terms of 8 query heads and their second terms, the 8
+//     columns positions; the two halves are added afterwards.  The contracted index may be taken
+//     in any order, so thread (g, t) of the second operand reads D / 4 dims of one row in one
+//     piece (16 or 8 bytes): k-step s takes its bytes 2s, 2s + 1.
+//   O^T = V^T P^T: the rows are 16 dims, the columns 8 query heads, so what S left in a thread
+//     (head g, two positions of each n-tile) is its piece of the second operand, and the products
+//     of both terms of P go into the same sums (a form with P as the first operand needs twice
+//     the registers for them).  Thread (g, t) reads one piece of 8 or 4 bytes of each of its 4
+//     positions, dims g D/8 ..; the pairs along positions that the operand needs are made by
 //     merging the nibbles of two rows before they are converted.
-//   A slot (n-tile i, column 2t + e) of S is position 8i + (e ? 7 - t : t) of a 16-position block:
-//     with it both kinds of shared-memory reads are free of bank conflicts.
+//   Column 2t + e of n-tile i of S is position 8i + (e ? 7 - t : t) of a 16-position block: with
+//     it both kinds of shared-memory reads are free of bank conflicts.
 constexpr int AT_WARPS = 4;
 constexpr int AT_TILE = 32;   // positions of a tile
-constexpr int AT_STAGES = 4;  // tiles of a warp in shared memory
+constexpr int AT_STAGES = 3;  // tiles of a warp in shared memory
+
+// The dim of column c of a split's sums: columns are ordered by m-tile, then g, then the pair.
+template <int D>
+__device__ __forceinline__ int dim_of(int c) {
+  return (c >> 1 & 7) * (D / 8) + 2 * (c >> 4) + (c & 1);
+}
 
 template <int D>
 struct TileBytes {
   static constexpr int codes = AT_TILE * D / 2, scales = AT_TILE * D / 16, all = 2 * (codes + scales);
 };
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {  // the rest of 16 B becomes 0
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// `bytes` of 16, the rest becomes 0
+__device__ __forceinline__ void cp_async16_part(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -71,6 +89,12 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ void mma_16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {  // c = A B
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -84,34 +108,57 @@ __device__ __forceinline__ int code_at(int r, int byte) {
   return D == 128 ? r * 64 + (byte ^ ((r & 2) << 4)) : r * 32 + byte;
 }
 
-// Rows [p0, p0 + 32) of one KV head into a stage; rows from p1 on are not read, their scales are 0.
+// Brings tiles of one KV head into a warp's stages.  A tile is one run of each of the four
+// buffers, so a lane's pieces lie at fixed distances from its pointers.  Only the last tile of a
+// split can be short: its rows from `nv` on are not read and their scales become 0.
 template <int D>
-__device__ __forceinline__ void load_tile(const AttendArgs& a, size_t row0, int p0, int p1, uint8_t* st, int lane) {
-  constexpr int CPR = D / 32, SPR = D / 16;  // 16-byte pieces of a row's codes, bytes of its scales
-  const size_t row = row0 + p0;
-  const int nv = p1 - p0;
-#pragma unroll
-  for (int e = 0; e < CPR; ++e) {
-    const int i = lane + 32 * e, r = i / CPR, c = i % CPR;
-    const int bytes = r < nv ? 16 : 0;
-    const size_t off = r < nv ? (row + r) * (D / 2) + c * 16 : row * (D / 2);
-    cp_async16(st + code_at<D>(r, c * 16), a.k_codes + off, bytes);
-    cp_async16(st + TileBytes<D>::codes + code_at<D>(r, c * 16), a.v_codes + off, bytes);
-  }
-  constexpr int SL = TileBytes<D>::scales / 16;  // lanes that bring the scales of K, and as many those of V
-  if (lane < 2 * SL) {
-    const int i = lane % SL;
-    const int bytes = min(16, max(0, nv * SPR - i * 16));
-    const uint8_t* src = (lane < SL ? a.k_scales : a.v_scales) + row * SPR + (bytes ? i * 16 : 0);
-    cp_async16(st + 2 * TileBytes<D>::codes + lane * 16, src, bytes);
-  }
-}
+struct TileLoader {
+  static constexpr int CPL = AT_TILE * D / 2 / 512;  // 16-byte pieces of a lane: 4 or 2, of 512 bytes each
+  static constexpr int SL = TileBytes<D>::scales / 16;  // lanes that bring the scales of K, and as many those of V
+  const uint8_t *k, *v, *s;
+  uint32_t c_dst, s_dst;
+  int lane;
 
-template <int D>
-__global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_kernel(const AttendArgs a) {
+  __device__ __forceinline__ void init(const AttendArgs& a, size_t row, uint8_t* ring, int lane_) {
+    lane = lane_;
+    k = a.k_codes + row * (D / 2) + lane * 16;
+    v = a.v_codes + row * (D / 2) + lane * 16;
+    s = (lane < SL ? a.k_scales : a.v_scales) + row * (D / 16) + (lane % SL) * 16;
+    c_dst = smem_u32(ring) + code_at<D>(lane * 16 / (D / 2), lane * 16 % (D / 2));
+    s_dst = smem_u32(ring) + 2 * TileBytes<D>::codes + lane * 16;
+  }
+  __device__ __forceinline__ void load(int stage, int nv) {
+    const uint32_t off = stage * TileBytes<D>::all;
+    if (nv >= AT_TILE) {
+#pragma unroll
+      for (int e = 0; e < CPL; ++e) {
+        cp_async16(c_dst + off + e * 512, k + e * 512);
+        cp_async16(c_dst + off + TileBytes<D>::codes + e * 512, v + e * 512);
+      }
+      if (lane < 2 * SL) cp_async16(s_dst + off, s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < CPL; ++e) {
+        const bool in = (lane * 16 + e * 512) / (D / 2) < nv;  // a piece lies in one row
+        cp_async16_part(c_dst + off + e * 512, in ? k + e * 512 : k - lane * 16, in ? 16 : 0);
+        cp_async16_part(c_dst + off + TileBytes<D>::codes + e * 512, in ? v + e * 512 : v - lane * 16, in ? 16 : 0);
+      }
+      if (lane < 2 * SL) {
+        const int first = (lane % SL) * 16, bytes = min(16, max(0, nv * (D / 16) - first));
+        cp_async16_part(s_dst + off, bytes ? s : s - first, bytes);
+      }
+    }
+    k += AT_WARPS * TileBytes<D>::codes;
+    v += AT_WARPS * TileBytes<D>::codes;
+    s += AT_WARPS * TileBytes<D>::scales;
+  }
+};
+
+template <int D, bool CLUSTER>
+__global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 4 : 5) kv4_split_kernel(const AttendArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
-  constexpr int KS = D / 16, NT = D / 8;  // k-steps of S, n-tiles of O
-  constexpr int OS = D + 8;               // floats of a head's row in the merge
+  constexpr int KS = D / 16;  // k-steps of S, m-tiles of O^T
+  constexpr int OS = D + 4;   // floats of a head's row in the merge
   pdl_launch_dependents();
   const int unit = blockIdx.y, split = blockIdx.x;
   const int hb = unit % a.nhb, g0 = (unit / a.nhb) % a.nkv, b = unit / (a.nhb * a.nkv);
@@ -119,6 +166,13 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
   const int n = seq_len(a, b);
   const int heads = min(HB, a.nrep - hb * HB);
   float* out = a.out + (size_t)b * a.ldo + (size_t)(g0 * a.nrep + hb * HB) * D;
+  float4 q[KS];  // on its way while the length is
+  {
+    const float* qp = a.q + (size_t)b * a.ldq + (size_t)(g0 * a.nrep + hb * HB + g) * D + t * (D / 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      q[s] = g < heads ? __ldg(reinterpret_cast<const float4*>(qp) + s) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   if (n <= 0) {
     if (n < 0 && tid == 0) record_error(a.err, VX_DEVICE_ERR_BOUNDS);
     if (split == 0)
@@ -126,14 +180,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
     return;
   }
   const int j0 = split * a.chunk, j1 = min(n, j0 + a.chunk);
-  if (j0 >= j1) return;
+  if (!CLUSTER && j0 >= j1) return;
   const size_t row0 = (size_t)(b * a.nkv + g0) * a.cap;
+  float* own_scores = reinterpret_cast<float*>(smem + AT_WARPS * AT_STAGES * TileBytes<D>::all);  // [chunk][8]
   uint8_t* ring = smem + warp * (AT_STAGES * TileBytes<D>::all);
   const int first = j0 + warp * AT_TILE;
   const int tiles = first < j1 ? (j1 - first + AT_WARPS * AT_TILE - 1) / (AT_WARPS * AT_TILE) : 0;
+  TileLoader<D> loader;
+  loader.init(a, row0 + first, ring, lane);
 #pragma unroll
   for (int i = 0; i < AT_STAGES - 1; ++i) {
-    if (i < tiles) load_tile<D>(a, row0, first + i * AT_WARPS * AT_TILE, j1, ring + i * TileBytes<D>::all, lane);
+    if (i < tiles) loader.load(i, j1 - (first + i * AT_WARPS * AT_TILE));
     cp_async_commit();
   }
 
@@ -142,14 +199,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
   uint32_t qh[KS][2], ql[KS][2];
   float mult;  // a sum of products times this is a base-2 score
   {
-    float4 q[KS];
     float amax = 0.f;
-    const float* qp = a.q + (size_t)b * a.ldq + (size_t)(g0 * a.nrep + hb * HB + g) * D + t * (D / 4);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      q[s] = g < heads ? __ldg(reinterpret_cast<const float4*>(qp) + s) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < KS; ++s)
       amax = fmaxf(amax, fmaxf(fmaxf(fabsf(q[s].x), fabsf(q[s].y)), fmaxf(fabsf(q[s].z), fabsf(q[s].w))));
-    }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const int e = (int)(__float_as_uint(amax) >> 23);  // 255: infinity, which gives NaN below
@@ -167,62 +220,81 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
     }
   }
 
-  float o[NT][4];
+  // m-tile i: dims g D/8 + 2i (numbers 0, 1) and + 1 (2, 3) of query heads 2t (0, 2) and 2t + 1 (1, 3)
+  float o[KS][4];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m = -INFINITY, l = 0.f;
-  // this lane's row of a 16-position block in S (columns of n-tile 0; + 8 of n-tile 1), its first in O
+  // byte offsets of this lane's pieces in a tile: its row of 8 positions in S, its two in O
   const int krow = (g & 1) ? 7 - (g >> 1) : (g >> 1);
+  const int k_off = code_at<D>(krow, t * (D / 8)), ks_off = 2 * TileBytes<D>::codes + krow * (D / 16) + t * (D / 64);
+  const int v_off[2] = {TileBytes<D>::codes + code_at<D>(t, g * (D / 16)),
+                        TileBytes<D>::codes + code_at<D>(7 - t, g * (D / 16))};
+  const int v_scales = 2 * TileBytes<D>::codes + TileBytes<D>::scales, v_group = g * (D / 8) / KV4_GROUP;
+  const int vs_off[2] = {v_scales + t * (D / 16) + v_group, v_scales + (7 - t) * (D / 16) + v_group};
 
   for (int it = 0; it < tiles; ++it) {
     cp_async_wait<AT_STAGES - 2>();
     __syncwarp();
     const int p0 = first + it * AT_WARPS * AT_TILE;
     const uint8_t* st = ring + (it % AT_STAGES) * TileBytes<D>::all;
-    const uint8_t *kc = st, *vc = st + TileBytes<D>::codes, *ks = st + 2 * TileBytes<D>::codes,
-                  *vs = ks + TileBytes<D>::scales;
     float s[8];  // n-tile i's columns 2t, 2t + 1 at 2i, 2i + 1
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + krow;
-      uint32_t w[KS / 2], sc[2];
-      if constexpr (D == 128) {
-        const uint4 v = *reinterpret_cast<const uint4*>(kc + code_at<D>(r, t * 16));
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        const uint32_t h = e4m3x2_to_h2(*reinterpret_cast<const uint16_t*>(ks + r * 8 + 2 * t));
-        sc[0] = __byte_perm(h, h, 0x1010);
-        sc[1] = __byte_perm(h, h, 0x3232);
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(kc + code_at<D>(r, t * 8));
-        w[0] = v.x, w[1] = v.y;
-        const uint32_t one = ks[r * 4 + t];
-        sc[0] = sc[1] = e4m3x2_to_h2(one | one << 8);
-      }
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i2 = 0; i2 < 2; ++i2) {  // two n-tiles at a time
+      uint32_t w[2][KS / 2], sc[2][2];
 #pragma unroll
-      for (int q = 0; q < KS / 2; ++q) {
-        uint32_t x[4];
-        e2m1x8_to_h2(w[q], x);
-        const uint32_t f = sc[q * 4 / KS];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = 2 * q + h;
-          mma_16816(c, qh[k][0], ql[k][0], qh[k][1], ql[k][1], mul_h2(x[2 * h], f), mul_h2(x[2 * h + 1], f));
+      for (int e = 0; e < 2; ++e) {
+        const uint8_t* p = st + (2 * i2 + e) * 8 * (D / 2);
+        const uint8_t* ps = st + (2 * i2 + e) * 8 * (D / 16);
+        if constexpr (D == 128) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p + k_off);
+          w[e][0] = v.x, w[e][1] = v.y, w[e][2] = v.z, w[e][3] = v.w;
+          const uint32_t h = e4m3x2_to_h2(*reinterpret_cast<const uint16_t*>(ps + ks_off));
+          sc[e][0] = __byte_perm(h, h, 0x1010);
+          sc[e][1] = __byte_perm(h, h, 0x3232);
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(p + k_off);
+          w[e][0] = v.x, w[e][1] = v.y;
+          const uint32_t one = ps[ks_off];
+          sc[e][0] = sc[e][1] = e4m3x2_to_h2(one | one << 8);
         }
       }
-      s[2 * i] = (c[0] + c[2]) * mult;
-      s[2 * i + 1] = (c[1] + c[3]) * mult;
+      float c[2][4];
+#pragma unroll
+      for (int q = 0; q < KS / 2; ++q) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t x[4];
+          e2m1x8_to_h2(w[e][q], x);
+          const uint32_t f = sc[e][q * 4 / KS];
+          if (q == 0)
+            mma_16816_zero(c[e], qh[0][0], ql[0][0], qh[0][1], ql[0][1], mul_h2(x[0], f), mul_h2(x[1], f));
+          else
+            mma_16816(c[e], qh[2 * q][0], ql[2 * q][0], qh[2 * q][1], ql[2 * q][1], mul_h2(x[0], f), mul_h2(x[1], f));
+          mma_16816(c[e], qh[2 * q + 1][0], ql[2 * q + 1][0], qh[2 * q + 1][1], ql[2 * q + 1][1], mul_h2(x[2], f),
+                    mul_h2(x[3], f));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * i2 + e;
+        s[2 * i] = (c[e][0] + c[e][2]) * mult;
+        s[2 * i + 1] = (c[e][1] + c[e][3]) * mult;
+      }
     }
     if (p0 + AT_TILE > j1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (p0 + 8 * (i >> 1) + ((i & 1) ? 7 - t : t) >= j1) s[i] = -INFINITY;
     }
-    if (a.scores) {
+    if (CLUSTER ? a.weights != nullptr : a.scores != nullptr) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int p = p0 + 8 * (i >> 1) + ((i & 1) ? 7 - t : t);
-        if (p < j1) a.scores[((size_t)unit * a.max_len + p) * HB + g] = s[i];
+        if (CLUSTER)
+          own_scores[(p - j0) * HB + g] = s[i];
+        else if (p < j1)
+          a.scores[((size_t)unit * a.max_len + p) * HB + g] = s[i];
       }
     }
     float mt = s[0];
@@ -236,10 +308,12 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
       const float mn = fmaxf(m, mt), alpha = ex2(m - mn);
       m = mn;
       l *= alpha;
+      const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] *= alpha;
+      for (int i = 0; i < KS; ++i) {
+        o[i][0] *= a0, o[i][2] *= a0;
+        o[i][1] *= a1, o[i][3] *= a1;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -259,20 +333,18 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
       uint32_t w[4][NW], sc[2];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {  // n-tile e / 2, column 2t + e % 2
-        const int r = 16 * k + 8 * (e >> 1) + ((e & 1) ? 7 - t : t);
+        const uint8_t* p = st + v_off[e & 1] + (2 * k + (e >> 1)) * 8 * (D / 2);
         if constexpr (D == 128) {
-          const uint2 v = *reinterpret_cast<const uint2*>(vc + code_at<D>(r, g * 8));
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
           w[e][0] = v.x, w[e][NW - 1] = v.y;
         } else {
-          w[e][0] = *reinterpret_cast<const uint32_t*>(vc + code_at<D>(r, g * 4));
+          w[e][0] = *reinterpret_cast<const uint32_t*>(p);
         }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int r0 = 16 * k + 8 * i + t, r1 = 16 * k + 8 * i + 7 - t;
-        const uint32_t s0 = D == 128 ? vs[r0 * 8 + g] : vs[r0 * 4 + (g >> 1)];
-        const uint32_t s1 = D == 128 ? vs[r1 * 8 + g] : vs[r1 * 4 + (g >> 1)];
-        sc[i] = e4m3x2_to_h2(s0 | s1 << 8);
+        const uint8_t* p = st + (2 * k + i) * 8 * (D / 16);
+        sc[i] = e4m3x2_to_h2((uint32_t)p[vs_off[0]] | (uint32_t)p[vs_off[1]] << 8);
       }
 #pragma unroll
       for (int q = 0; q < NW; ++q) {
@@ -285,15 +357,16 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          mma_16816(o[8 * q + 2 * j], ph[0], pl[0], ph[1], pl[1], mul_h2(ev[0][j], sc[0]), mul_h2(ev[1][j], sc[1]));
-          mma_16816(o[8 * q + 2 * j + 1], ph[0], pl[0], ph[1], pl[1], mul_h2(od[0][j], sc[0]), mul_h2(od[1][j], sc[1]));
+          const uint32_t a0 = mul_h2(ev[0][j], sc[0]), a1 = mul_h2(od[0][j], sc[0]), a2 = mul_h2(ev[1][j], sc[1]),
+                         a3 = mul_h2(od[1][j], sc[1]);
+          mma_16816(o[4 * q + j], a0, a1, a2, a3, ph[0], ph[1]);
+          mma_16816(o[4 * q + j], a0, a1, a2, a3, pl[0], pl[1]);
         }
       }
     }
     __syncwarp();  // every lane has read the stage that the next load goes into
     const int nx = it + AT_STAGES - 1;
-    if (nx < tiles)
-      load_tile<D>(a, row0, first + nx * AT_WARPS * AT_TILE, j1, ring + (nx % AT_STAGES) * TileBytes<D>::all, lane);
+    if (nx < tiles) loader.load(nx % AT_STAGES, j1 - (first + nx * AT_WARPS * AT_TILE));
     cp_async_commit();
   }
   cp_async_wait<0>();
@@ -301,145 +374,295 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 3 : 4) kv4_split_ker
   l += __shfl_xor_sync(0xffffffffu, l, 2);
   __syncthreads();  // the rings are free
 
-  // merge the warps: column c = 8j + column of n-tile j of a head's row is dim (c % 8) D/8 + c / 8
-  float* so = reinterpret_cast<float*>(smem);          // [warps][8][OS]
-  float* sml = so + AT_WARPS * HB * OS;                 // [warps][8][2]
+  // merge the warps: column c of a head's row is dim_of<D>(c), the order in which threads hold them
+  float* so = reinterpret_cast<float*>(smem);  // [warps][8][OS]
+  float* sml = so + AT_WARPS * HB * OS;         // [warps][8][2]
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
-    *reinterpret_cast<float2*>(so + (warp * HB + g) * OS + j * 8 + 2 * t) =
-        make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
+  for (int i = 0; i < KS; ++i) {
+    float* p = so + (warp * HB + 2 * t) * OS + i * 16 + 2 * g;
+    *reinterpret_cast<float2*>(p) = make_float2(o[i][0], o[i][2]);
+    *reinterpret_cast<float2*>(p + OS) = make_float2(o[i][1], o[i][3]);
+  }
   if (t == 0) {
     sml[(warp * HB + g) * 2] = m;
     sml[(warp * HB + g) * 2 + 1] = l;
   }
   __syncthreads();
-  for (int i = tid; i < heads * D; i += AT_WARPS * 32) {
-    const int h = i / D, c = i % D;
-    float M = -INFINITY, L = 0.f, x = 0.f;
+  float* joined = sml + AT_WARPS * HB * 2;  // [8][2]: maximum and sum of this block
+  for (int i = tid; i < heads * (D / 4); i += AT_WARPS * 32) {
+    const int h = i / (D / 4), c = i % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int w = 0; w < AT_WARPS; ++w) M = fmaxf(M, sml[(w * HB + h) * 2]);
+    const float M0 = CLUSTER && j0 >= j1 ? 0.f : M;  // a block without positions: all zeros
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < AT_WARPS; ++w) {
-      const float f = ex2(sml[(w * HB + h) * 2] - M);
+      const float f = ex2(sml[(w * HB + h) * 2] - M0);
+      const float4 y = *reinterpret_cast<const float4*>(so + (w * HB + h) * OS + c);
       L = fmaf(f, sml[(w * HB + h) * 2 + 1], L);
-      x = fmaf(f, so[(w * HB + h) * OS + c], x);
+      x.x = fmaf(f, y.x, x.x);
+      x.y = fmaf(f, y.y, x.y);
+      x.z = fmaf(f, y.z, x.z);
+      x.w = fmaf(f, y.w, x.w);
     }
-    if (a.nsplit == 1)
-      out[h * D + (c % 8) * (D / 8) + c / 8] = x / L;
+    if (a.nsplit == 1) {
+      *reinterpret_cast<float2*>(out + h * D + dim_of<D>(c)) = make_float2(x.x / L, x.y / L);
+      *reinterpret_cast<float2*>(out + h * D + dim_of<D>(c + 2)) = make_float2(x.z / L, x.w / L);
+    } else if (CLUSTER) {
+      *reinterpret_cast<float4*>(so + h * OS + c) = x;  // read by this thread alone before
+    } else {
+      *reinterpret_cast<float4*>(a.part_o + (((size_t)unit * a.nsplit + split) * HB + h) * D + c) = x;
+    }
+    if (c == 0) {
+      if (CLUSTER)
+        *reinterpret_cast<float2*>(joined + h * 2) = make_float2(M, L);
+      else if (a.part_ml)
+        *reinterpret_cast<float2*>(a.part_ml + (((size_t)unit * a.nsplit + split) * HB + h) * 2) = make_float2(M, L);
+    }
+  }
+  if constexpr (CLUSTER) {
+    // join the splits: each block of the cluster takes a part of the columns
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = a.nsplit, rank = (int)cl.block_rank();
+    if (C > 1)
+      cl.sync();
     else
-      a.part_o[(((size_t)unit * a.nsplit + split) * HB + h) * D + c] = x;
-    if (c == 0 && a.part_ml) {
-      float* p = a.part_ml + (((size_t)unit * a.nsplit + split) * HB + h) * 2;
-      p[0] = M;
-      p[1] = L;
+      __syncthreads();
+    float* fin = joined + HB * 2;  // [8][2]: maximum and 1 / sum over the cluster
+    if (tid < heads) {  // where the weights or other blocks' sums need it
+      float M = -INFINITY, L = 0.f;
+      for (int r = 0; r < C; ++r) M = fmaxf(M, cl.map_shared_rank(joined, r)[tid * 2]);
+      for (int r = 0; r < C; ++r) {
+        const float* p = cl.map_shared_rank(joined, r) + tid * 2;
+        L = fmaf(ex2(p[0] - M), p[1], L);
+      }
+      fin[tid * 2] = M;
+      fin[tid * 2 + 1] = 1.f / L;
     }
+    __syncthreads();
+    for (int i = rank * AT_WARPS * 32 + tid; C > 1 && i < heads * (D / 4); i += C * AT_WARPS * 32) {
+      const int h = i / (D / 4), c = i % (D / 4) * 4;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int r = 0; r < C; ++r) {
+        const float f = ex2(cl.map_shared_rank(joined, r)[h * 2] - fin[h * 2]);
+        const float4 y = *reinterpret_cast<const float4*>(cl.map_shared_rank(so, r) + h * OS + c);
+        x.x = fmaf(f, y.x, x.x);
+        x.y = fmaf(f, y.y, x.y);
+        x.z = fmaf(f, y.z, x.z);
+        x.w = fmaf(f, y.w, x.w);
+      }
+      const float inv = fin[h * 2 + 1];
+      *reinterpret_cast<float2*>(out + h * D + dim_of<D>(c)) = make_float2(x.x * inv, x.y * inv);
+      *reinterpret_cast<float2*>(out + h * D + dim_of<D>(c + 2)) = make_float2(x.z * inv, x.w * inv);
+    }
+    if (a.weights) {  // one block of query heads alone: a row's weight is this block's to write
+      for (int j = j0 + tid; j < j1; j += AT_WARPS * 32) {
+        const float4* p = reinterpret_cast<const float4*>(own_scores + (j - j0) * HB);
+        const float4 x = p[0], y = p[1];
+        const float sc[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        float w = 0.f;
+#pragma unroll
+        for (int h = 0; h < HB; ++h)
+          if (h < heads) w += ex2(sc[h] - fin[h * 2]) * fin[h * 2 + 1];
+        a.weights[row0 + j] += w;
+      }
+    }
+    if (C > 1) cl.sync();  // the other blocks have read this one's sums
   }
 }
 
 // Maximum and 1 / sum of one head over the active splits, by one warp.
 __device__ __forceinline__ void head_stats(const AttendArgs& a, int unit, int r, int active, float* M, float* inv) {
   const int lane = threadIdx.x & 31;
-  const float* p = a.part_ml + ((size_t)unit * a.nsplit * HB + r) * 2;
+  const float2* p = reinterpret_cast<const float2*>(a.part_ml) + (size_t)unit * a.nsplit * HB + r;
   float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < active; s += 32) m = fmaxf(m, p[(size_t)s * HB * 2]);
-  m = warp_max(m);
-  for (int s = lane; s < active; s += 32) l += p[(size_t)s * HB * 2 + 1] * ex2(p[(size_t)s * HB * 2] - m);
-  *M = m;
-  *inv = 1.f / warp_sum(l);
+  for (int s = lane; s < active; s += 32) {  // each lane's own running maximum, joined below
+    const float2 x = p[(size_t)s * HB];
+    const float mn = fmaxf(m, x.x);
+    l = l * ex2(m - mn) + x.y * ex2(x.x - mn);
+    m = mn;
+  }
+  *M = warp_max(m);
+  *inv = 1.f / warp_sum(l * ex2(m - *M));
 }
 
-// Blocks 0 .. units * 8 - 1 merge one head each (where there is more than one split); the blocks
-// behind them add the probabilities of 256 positions of one KV head to its weights.
+// The first units * 8 * slices blocks merge a head's columns (where there is more than one split),
+// D / slices of them: D / slices / 4 lanes read a split's, and the block's groups of lanes take
+// other splits.  The blocks behind them add the probabilities of a run of positions of one KV head
+// to its weights, FIN_POS to a thread.
+constexpr int FIN_POS = 2;
+
 template <int D>
-__global__ void __launch_bounds__(256) kv4_finish_kernel(const AttendArgs a, int merge_blocks, int chunks) {
-  __shared__ float sm[HB * 2];
+__global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, int slices, int merge_blocks, int chunks) {
+  extern __shared__ __align__(16) float4 acc[];  // one for each thread
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((int)blockIdx.x < merge_blocks) {
-    const int unit = blockIdx.x / HB, r = blockIdx.x % HB;
+    const int slice = blockIdx.x % slices, r = blockIdx.x / slices % HB, unit = blockIdx.x / (slices * HB);
     const int hb = unit % a.nhb, g = (unit / a.nhb) % a.nkv, b = unit / (a.nhb * a.nkv);
     const int n = seq_len(a, b);
     if (n <= 0 || hb * HB + r >= a.nrep) return;
     const int active = (n + a.chunk - 1) / a.chunk;
-    __shared__ float acc[8][D];
+    const int lps = D / 4 / slices, groups = blockDim.x / lps, grp = tid / lps, l4 = slice * lps + tid % lps;
     float M, inv;
     head_stats(a, unit, r, active, &M, &inv);
-    constexpr int DPL = D / 32;
-    float o[DPL] = {};
-    for (int s = warp; s < active; s += 8) {
-      const float f = ex2(a.part_ml[(((size_t)unit * a.nsplit + s) * HB + r) * 2] - M);
-      const float* po = a.part_o + (((size_t)unit * a.nsplit + s) * HB + r) * D + lane * DPL;
-      for (int e = 0; e < DPL; ++e) o[e] = fmaf(f, po[e], o[e]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* ml = a.part_ml + ((size_t)unit * a.nsplit * HB + r) * 2;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + ((size_t)unit * a.nsplit * HB + r) * D) + l4;
+#pragma unroll 4
+    for (int s = grp; s < active; s += groups) {
+      const float f = ex2(ml[(size_t)s * HB * 2] - M);
+      const float4 x = po[(size_t)s * HB * (D / 4)];
+      o.x = fmaf(f, x.x, o.x);
+      o.y = fmaf(f, x.y, o.y);
+      o.z = fmaf(f, x.z, o.z);
+      o.w = fmaf(f, x.w, o.w);
     }
-    for (int e = 0; e < DPL; ++e) acc[warp][lane * DPL + e] = o[e];
-    __syncthreads();
-    if ((int)threadIdx.x < D) {
-      float t = 0.f;
-      for (int w = 0; w < 8; ++w) t += acc[w][threadIdx.x];
-      const int c = threadIdx.x;  // the splits' columns are in the order of their n-tiles
-      a.out[(size_t)b * a.ldo + (size_t)(g * a.nrep + hb * HB + r) * D + (c % 8) * (D / 8) + c / 8] = t * inv;
+    acc[tid] = o;
+    for (int half = groups / 2; half > 0; half /= 2) {  // the groups, two by two
+      __syncthreads();
+      if (grp < half) {
+        const float4 x = acc[tid + half * lps];
+        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+        acc[tid] = o;
+      }
+    }
+    if (grp == 0) {
+      float* out = a.out + (size_t)b * a.ldo + (size_t)(g * a.nrep + hb * HB + r) * D;
+      *reinterpret_cast<float2*>(out + dim_of<D>(l4 * 4)) = make_float2(o.x * inv, o.y * inv);
+      *reinterpret_cast<float2*>(out + dim_of<D>(l4 * 4 + 2)) = make_float2(o.z * inv, o.w * inv);
     }
     return;
   }
+  float* sm = reinterpret_cast<float*>(acc);  // [8][2]
   const int i = blockIdx.x - merge_blocks;
   const int c = i % chunks, bg = i / chunks, b = bg / a.nkv;
-  const int n = seq_len(a, b);
-  if (n <= 0 || c * 256 >= n) return;
+  const int n = seq_len(a, b), j0 = c * FIN_POS * (int)blockDim.x + tid;
+  if (n <= 0 || j0 - tid >= n) return;
   const int active = (n + a.chunk - 1) / a.chunk;
-  const int j = c * 256 + threadIdx.x;
-  float w = 0.f;
+  float w[FIN_POS], got[FIN_POS];
+#pragma unroll
+  for (int u = 0; u < FIN_POS; ++u) {
+    const int j = j0 + u * blockDim.x;
+    w[u] = j < n ? a.weights[(size_t)bg * a.cap + j] : 0.f;
+    got[u] = 0.f;
+  }
   for (int hb = 0; hb < a.nhb; ++hb) {
     const int unit = bg * a.nhb + hb, heads = min(HB, a.nrep - hb * HB);
+    float4 s[FIN_POS][2];
+#pragma unroll
+    for (int u = 0; u < FIN_POS; ++u) {
+      const int j = min(j0 + u * (int)blockDim.x, n - 1);
+      const float4* p = reinterpret_cast<const float4*>(a.scores + ((size_t)unit * a.max_len + j) * HB);
+      s[u][0] = p[0];
+      s[u][1] = p[1];
+    }
     __syncthreads();
-    if (warp < heads) {
+    for (int h = warp; h < heads; h += blockDim.x / 32) {
       float M, inv;
-      head_stats(a, unit, warp, active, &M, &inv);
+      head_stats(a, unit, h, active, &M, &inv);
       if (lane == 0) {
-        sm[warp * 2] = M;
-        sm[warp * 2 + 1] = inv;
+        sm[h * 2] = M;
+        sm[h * 2 + 1] = inv;
       }
     }
     __syncthreads();
-    if (j < n) {
-      const float* s = a.scores + ((size_t)unit * a.max_len + j) * HB;
-      for (int r = 0; r < heads; ++r) w += ex2(s[r] - sm[r * 2]) * sm[r * 2 + 1];
+#pragma unroll
+    for (int u = 0; u < FIN_POS; ++u) {
+      const float x[8] = {s[u][0].x, s[u][0].y, s[u][0].z, s[u][0].w, s[u][1].x, s[u][1].y, s[u][1].z, s[u][1].w};
+#pragma unroll
+      for (int h = 0; h < HB; ++h)
+        if (h < heads) got[u] += ex2(x[h] - sm[h * 2]) * sm[h * 2 + 1];
     }
   }
-  if (j < n) a.weights[(size_t)bg * a.cap + j] += w;
+#pragma unroll
+  for (int u = 0; u < FIN_POS; ++u) {
+    const int j = j0 + u * blockDim.x;
+    if (j < n) a.weights[(size_t)bg * a.cap + j] = w[u] + got[u];
+  }
 }
+
+constexpr int AT_MAX_CLUSTER = 8;    // splits that a cluster joins
+constexpr int AT_CLUSTER_CHUNK = 512;  // their positions at most: the scores of a tracking call lie in shared memory
 
 struct AttendPlan {
   int nhb, chunk, nsplit;
+  bool cluster;
   size_t ml_bytes, o_bytes, score_bytes;
+  size_t need() const { return ml_bytes + o_bytes + score_bytes; }
 };
 
 AttendPlan plan_of(const vx_kv4* c, int nh, int max_len, int track) {
-  AttendPlan p;
+  AttendPlan p = {};
+  constexpr int kLeast = AT_WARPS * AT_TILE;  // a tile for each warp
   const int nrep = nh / c->n_kv_heads;
   p.nhb = (nrep + HB - 1) / HB;
   const long long units = (long long)c->batch * c->n_kv_heads * p.nhb;
-  // about eight rounds of three blocks per SM, a tile of each warp at least
-  constexpr long long kLeast = AT_WARPS * AT_TILE;
-  long long chunk = (units * max_len + 148 * 24 - 1) / (148 * 24);
-  chunk = std::min<long long>(2048, (chunk + kLeast - 1) / kLeast * kLeast);
-  chunk = std::max(chunk, kLeast);
+  // short sequences: the most splits, as long as all blocks are on the GPU at once (four to an SM)
+  auto chunk_of = [&](int splits) { return std::max(1, (max_len + splits * kLeast - 1) / (splits * kLeast)) * kLeast; };
+  int splits = AT_MAX_CLUSTER;
+  while (splits > 1 && (units * splits > 148 * 4 || (splits / 2) * kLeast >= max_len) && chunk_of(splits / 2) <= AT_CLUSTER_CHUNK)
+    splits /= 2;
+  // (several blocks of query heads would add to the same weights: not in a cluster)
+  if (chunk_of(splits) <= AT_CLUSTER_CHUNK && p.nhb == 1) {
+    p.cluster = true;
+    p.chunk = chunk_of(splits);
+    p.nsplit = splits;
+    return p;
+  }
+  long long chunk = (units * max_len + 148 * 8 - 1) / (148 * 8);
+  const long long least = units * max_len <= 148 * 4 * kLeast ? kLeast : 512;
+  chunk = std::min<long long>(4096, std::max(least, (chunk + kLeast - 1) / kLeast * kLeast));
   p.chunk = (int)chunk;
   p.nsplit = std::max(1, (int)((max_len + chunk - 1) / chunk));
-  const bool parts = p.nsplit > 1 || track;
-  p.ml_bytes = parts ? (size_t)units * p.nsplit * HB * 2 * 4 : 0;
+  p.ml_bytes = p.nsplit > 1 || track ? (size_t)units * p.nsplit * HB * 2 * 4 : 0;
   p.o_bytes = p.nsplit > 1 ? (size_t)units * p.nsplit * HB * c->head_dim * 4 : 0;
   p.score_bytes = track ? (size_t)units * max_len * HB * 4 : 0;
   return p;
 }
 
+constexpr size_t split_smem(int d) { return AT_WARPS * AT_STAGES * (d == 128 ? TileBytes<128>::all : TileBytes<64>::all); }
+constexpr size_t cluster_smem(int d, int chunk, bool track) {
+  return split_smem(d) + (track ? (size_t)chunk * HB * 4 : 0);
+}
+
+template <int D>
+cudaError_t launch_split(const AttendArgs& a, const AttendPlan& p, int units, cudaStream_t st) {
+  if (!p.cluster) {
+    kv4_split_kernel<D, false><<<dim3(p.nsplit, units), AT_WARPS * 32, split_smem(D), st>>>(a);
+    return cudaGetLastError();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.nsplit, units);
+  cfg.blockDim = dim3(AT_WARPS * 32);
+  cfg.dynamicSmemBytes = cluster_smem(D, p.chunk, a.weights != nullptr);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.nsplit;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.nsplit > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kv4_split_kernel<D, true>, a);
+}
+
+template <int D>
+cudaError_t configure_split() {
+  const cudaError_t e = cudaFuncSetAttribute(kv4_split_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)split_smem(D));
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(kv4_split_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              (int)cluster_smem(D, AT_CLUSTER_CHUNK, true));
+}
+
 }  // namespace
 
 cudaError_t kv4_attend_configure() {
-  const cudaError_t e = cudaFuncSetAttribute(kv4_split_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             AT_WARPS * AT_STAGES * TileBytes<128>::all);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(kv4_split_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              AT_WARPS * AT_STAGES * TileBytes<64>::all);
+  const cudaError_t e = configure_split<128>();
+  return e != cudaSuccess ? e : configure_split<64>();
 }
 
 }  // namespace vx
@@ -450,8 +673,7 @@ extern "C" {
 
 size_t vx_kv4_attend_workspace(const vx_kv4* c, int nh, int max_len, int track) {
   if (!c || c->n_kv_heads <= 0 || nh <= 0 || nh % c->n_kv_heads != 0 || max_len < 0 || c->batch <= 0) return 0;
-  const AttendPlan p = plan_of(c, nh, max_len, track);
-  return p.ml_bytes + p.o_bytes + p.score_bytes;
+  return plan_of(c, nh, max_len, track).need();
 }
 
 int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* c, const float* q, int64_t q_stride, int nh, const int32_t* lens,
@@ -470,7 +692,7 @@ int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* c, const float* q, int64_t q_stride
       q_stride < (int64_t)nh * c->head_dim || out_stride < (int64_t)nh * c->head_dim)
     return fail(ctx, VX_ERR_ARG, "kv4_attend: q and out must be 16-byte aligned rows of nh * head_dim floats");
   const AttendPlan p = plan_of(c, nh, max_len, track);
-  const size_t need = p.ml_bytes + p.o_bytes + p.score_bytes;
+  const size_t need = p.need();
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
     return fail(ctx, VX_ERR_ARG, "kv4_attend: %zu bytes of 16-byte aligned workspace are needed", need);
   DeviceGuard guard(ctx->device);
@@ -503,17 +725,17 @@ int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* c, const float* q, int64_t q_stride
   const int units = a.B * a.nkv * a.nhb;
   if (units > 65535) return fail(ctx, VX_ERR_SHAPE, "kv4_attend: more than 65535 blocks of 8 query heads");
   count_launch();
-  if (c->head_dim == 128)
-    kv4_split_kernel<128><<<dim3(p.nsplit, units), AT_WARPS * 32, AT_WARPS * AT_STAGES * TileBytes<128>::all, st>>>(a);
-  else
-    kv4_split_kernel<64><<<dim3(p.nsplit, units), AT_WARPS * 32, AT_WARPS * AT_STAGES * TileBytes<64>::all, st>>>(a);
-  VX_CUDA(ctx, cudaGetLastError());
+  VX_CUDA(ctx, c->head_dim == 128 ? launch_split<128>(a, p, units, st) : launch_split<64>(a, p, units, st));
   if (!need || max_len == 0) return VX_OK;
-  const int merge = p.nsplit > 1 ? units * HB : 0, chunks = (max_len + 255) / 256;
-  PdlLaunch pl(dim3(merge + (track ? a.B * a.nkv * chunks : 0)), dim3(256), 0, st);
+  // few units with many splits: more blocks to a head, and more groups of lanes in them
+  const int slices = units <= 16 ? c->head_dim / 32 : 1;
+  int threads = 256;
+  while (threads < 1024 && threads / (c->head_dim / 4 / slices) * 4 < p.nsplit) threads *= 2;
+  const int merge = p.nsplit > 1 ? units * HB * slices : 0, chunks = (max_len + FIN_POS * threads - 1) / (FIN_POS * threads);
+  PdlLaunch pl(dim3(merge + (track ? a.B * a.nkv * chunks : 0)), dim3(threads), threads * sizeof(float4), st);
   count_launch();
-  VX_CUDA(ctx, c->head_dim == 128 ? cudaLaunchKernelEx(&pl.cfg, kv4_finish_kernel<128>, a, merge, chunks)
-                                  : cudaLaunchKernelEx(&pl.cfg, kv4_finish_kernel<64>, a, merge, chunks));
+  VX_CUDA(ctx, c->head_dim == 128 ? cudaLaunchKernelEx(&pl.cfg, kv4_finish_kernel<128>, a, slices, merge, chunks)
+                                  : cudaLaunchKernelEx(&pl.cfg, kv4_finish_kernel<64>, a, slices, merge, chunks));
   return VX_OK;
 }
 
