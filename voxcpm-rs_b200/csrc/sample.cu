@@ -5,10 +5,20 @@
 // A token's weight is w = rint(exp((l - lmax) / T) * 2^44) as a 64-bit integer: sums of weights
 // are exact whatever their order (a row of 2^18 tokens stays below 2^62), so every block and
 // every order of atomics finds the same border.  The tokens that stay are a prefix of the order
-// (logit descending, index ascending), described by the key of its last logit and how many
-// tokens of that key stay; radix passes over the ordered keys find it, by count for top-k, by
-// weight for top-p.  The draw takes the first token in index order whose running sum of staying
-// weights exceeds u * total.
+// (logit descending, index ascending), described by the last of them, an "entry": the logit's
+// ordered bits above the inverted index.
+//
+// The border is found by counts (top-k) or weights (top-p): a histogram of lmax - l in 2048 equal
+// buckets says in which bucket it lies, and the few entries of that bucket are gathered, sorted
+// and summed by one block.  Where top-k leaves few tokens these are gathered at once, and top-p,
+// min-p and the draw work on the sorted list.  A bucket too full for the list (equal logits, or a
+// border behind the range of the buckets) goes through radix passes over the entries instead.
+// The draw takes the first token in index order whose running sum of staying weights exceeds
+// u * total: sums of each warp's part of the row, then one warp walks its part again.
+//
+// What bounds it: f64 arithmetic and shared-memory atomics where every token needs its weight
+// (5.8 clocks of an SM for 32 exponentials, 3.7 for their two 32-bit atomics; one 64-bit atomic is
+// a compare-and-swap loop of 30), else the latency of four cluster barriers.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -23,11 +33,15 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int SP_THREADS = 1024;
+constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32;
 constexpr int SP_MAX_CLUSTER = 8;
-constexpr int SP_SLICE = 32768;       // logits of a block: 128 KB
-constexpr int SP_MAX_VOCAB = 1 << 18;
-constexpr double SP_ONE = 17592186044416.0;  // 2^44
+constexpr int SP_SLICE = 32768;      // logits of a block at most: 128 KB
+constexpr int SP_MAX_VOCAB = SP_SLICE * SP_MAX_CLUSTER;
+constexpr int SP_BUCKETS = 2048, SP_COARSE = 64;
+constexpr int SP_LIST = 1024;        // entries that are sorted
+constexpr int SP_BITS = 44;          // binary places of a weight
+constexpr double SP_ONE = (double)(1ull << SP_BITS);
+static_assert(SP_MAX_VOCAB == 1 << 18, "the vocabulary that the header names; sums stay below 2^62");
 
 struct SampleArgs {
   const float* logits;
@@ -40,266 +54,479 @@ struct SampleArgs {
   float* logprob;
 };
 
-// ascending with the logit; -0 and 0 are the same
-__device__ __forceinline__ uint32_t key_of(float l) {
-  const uint32_t u = __float_as_uint(l + 0.f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// Ascending with the logit, then descending with the index; -0 and 0 are the same.
+__device__ __forceinline__ u64 entry_of(float l, int index) {
+  const uint32_t u = __float_as_uint(l + 0.f), k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return (u64)k << 24 | (0xffffffu - (uint32_t)index);
 }
-__device__ __forceinline__ float logit_of(uint32_t k) {
+__device__ __forceinline__ float logit_of(u64 entry) {
+  const uint32_t k = (uint32_t)(entry >> 24);
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+__device__ __forceinline__ int index_of(u64 entry) { return 0xffffff - (int)(entry & 0xffffffu); }
 
-__device__ __forceinline__ u64 weight_of(float l, float lmax, double T) {
-  if (l == lmax) return (u64)SP_ONE;
-  const double z = ((double)l - (double)lmax) / T;
-  // below exp(-31.2) 2^44 = 1/2 a weight is 0; so is that of -inf (or anything next to +inf) at T = inf, a NaN here
-  return z > -31.5 ? __double2ull_rn(exp(z) * SP_ONE) : 0;
-}
+struct SampleShared {
+  union {
+    struct {
+      uint32_t lo[SP_BUCKETS], hi[SP_BUCKETS];
+    } hist;
+    struct {
+      u64 wt[SP_LIST], pre[SP_LIST];  // of the sorted list: weights, running sums
+    } list;
+  };
+  u64 ent[SP_LIST];  // gathered entries
+  double tab[64];    // 2^(i / 64)
+  u64 coarse[SP_COARSE];
+  u64 warp64[SP_WARPS];
+  u64 total, above, border;
+  uint32_t warp32[SP_WARPS];
+  float fmax, fmin;
+  int bad, bucket, n;
+};
+
+// Everything that the passes over a row share.
+struct Row {
+  const float* x;  // this block's logits
+  int lo, cnt;     // their first index and number
+  float lmax;
+  double lmax_d, inv_t;
+  const double* tab;
+
+  // exp by a table of 2^(i/64) and a polynomial of degree 4 (table-driven, after Tang, 1989): off by
+  // less than 2^-43 of itself.  A token at z <= -31.5 has no weight (exp(-31.2) 2^44 = 1/2), nor has
+  // one next to +infinity or -infinity itself, where z is infinite or a NaN.
+  __device__ __forceinline__ u64 weight(float l) const {
+    if (l == lmax) return 1ull << SP_BITS;
+    const double z = ((double)l - lmax_d) * inv_t;
+    if (!(z > -31.5)) return 0;
+    constexpr double kShift = 6755399441055744.0;                   // 1.5 * 2^52: rounds to an integer
+    const double t = fma(z, 92.332482616893656877, kShift);         // 64 / ln 2
+    const int n = __double2loint(t);
+    const double r = fma(t - kShift, -0.010830424696249145, z);     // ln 2 / 64; |r| <= 0.0055
+    double p = fma(r, 1.0 / 24, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    p *= tab[n & 63];
+    const double s = __hiloint2double(__double2hiint(p) + (((n >> 6) + SP_BITS) << 20), __double2loint(p));
+    return (u64)__double_as_longlong(s + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52: to the nearest integer
+  }
+};
 
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-struct SampleShared {
-  u64 mass[2][256], tot[256];
-  u64 warp64[32], part64[2];
-  uint32_t warp32[32], part32[4];
-  u64 left;
-  uint32_t prefix;
-  float fmax;
-  int bad;
-};
-
-// Block-wide sums; every thread gets the total.
-__device__ __forceinline__ u64 block_sum64(u64 v, u64* red) {
-  v = warp_sum64(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  u64 t = 0;
-  for (int w = 0; w < SP_THREADS / 32; ++w) t += red[w];
-  return t;
+__device__ __forceinline__ u64 warp_scan64(u64 v) {  // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
 }
 
-// The largest key T with sum(value of tokens with key >= T) >= need; *left = need minus the sum
-// of those above T.  value(key) is summed over this cluster's tokens.
-template <class F>
-__device__ uint32_t radix_find(cg::cluster_group& cl, SampleShared& s, const float* x, int cnt, u64 need, u64* left,
-                               F value) {
+// Adds to a 64-bit sum in two words; the word of the carry is touched where there is something to add.
+__device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, u64 v) {
+  const uint32_t l = (uint32_t)v, old = atomicAdd(lo, l);
+  const uint32_t h = (uint32_t)(v >> 32) + (old + l < l);
+  if (h) atomicAdd(hi, h);
+}
+
+// Equal buckets of lmax - l: at `per` buckets to a unit, the last one holds the rest.
+struct Buckets {
+  float lmax, per;
+  __device__ __forceinline__ int operator()(float l) const {
+    return l == lmax ? 0 : (int)fminf((lmax - l) * per, (float)(SP_BUCKETS - 1));
+  }
+};
+
+// The histogram over the cluster of value(l, index) and the bucket in which the running sum from
+// the largest logit on reaches need(total): s.bucket, s.above (the sum before it), s.total.  Every
+// block finds the same.
+template <class Value, class Need>
+__device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& row, const Buckets& bucket, bool wide,
+                            Value value, Need need) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = (int)cl.num_blocks();
-  uint32_t prefix = 0;
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    u64* h = s.mass[pass & 1];
-    cl.sync();  // every block is done with what it read of the pass before last
-    if (tid < 256) h[tid] = 0;
-    __syncthreads();
-    for (int j = tid; j < cnt; j += SP_THREADS) {
-      const uint32_t k = key_of(x[j]);
-      if (pass == 0 || (k >> (shift + 8)) == (prefix >> (shift + 8))) {
-        const u64 v = value(x[j], k);
-        if (v) atomicAdd(&h[(k >> shift) & 255], v);
+  for (int i = tid; i < SP_BUCKETS; i += SP_THREADS) s.hist.lo[i] = s.hist.hi[i] = 0;
+  __syncthreads();
+  if (wide) {
+    for (int j = tid; j < row.cnt; j += SP_THREADS) {
+      const float l = row.x[j];
+      const u64 v = value(l, row.lo + j);
+      if (v) {
+        const int b = bucket(l);
+        add64(&s.hist.lo[b], &s.hist.hi[b], v);
       }
+    }
+  } else {
+    for (int j = tid; j < row.cnt; j += SP_THREADS) {
+      const float l = row.x[j];
+      if (l != -INFINITY) atomicAdd(&s.hist.lo[bucket(l)], 1u);
+    }
+  }
+  __syncthreads();
+  for (int c = warp; c < SP_COARSE; c += SP_WARPS) {
+    const int i = c * (SP_BUCKETS / SP_COARSE) + lane;
+    const u64 v = warp_sum64((u64)s.hist.hi[i] << 32 | s.hist.lo[i]);
+    if (lane == 0) s.coarse[c] = v;
+  }
+  cl.sync();
+  if (warp == 0) {
+    u64 v[2] = {0, 0};
+    for (int r = 0; r < C; ++r) {
+      const u64* p = cl.map_shared_rank(s.coarse, r) + lane * 2;
+      v[0] += p[0], v[1] += p[1];
+    }
+    const u64 incl = warp_scan64(v[0] + v[1]), total = __shfl_sync(0xffffffffu, incl, 31), want = need(total);
+    const uint32_t hit = __ballot_sync(0xffffffffu, incl >= want);
+    const int at = hit ? __ffs(hit) - 1 : 31;  // (always one: want is at most the total)
+    u64 above = incl - v[0] - v[1];
+    int c = lane * 2;
+    if (above + v[0] < want) above += v[0], ++c;
+    above = __shfl_sync(0xffffffffu, above, at);
+    c = __shfl_sync(0xffffffffu, c, at);
+    u64 f = 0;
+    const int i = c * (SP_BUCKETS / SP_COARSE) + lane;
+    for (int r = 0; r < C; ++r)
+      f += (u64)cl.map_shared_rank(s.hist.hi, r)[i] << 32 | cl.map_shared_rank(s.hist.lo, r)[i];
+    const u64 fi = warp_scan64(f) + above;
+    const uint32_t fh = __ballot_sync(0xffffffffu, fi >= want);
+    const int b = fh ? __ffs(fh) - 1 : 31;
+    const u64 before = __shfl_sync(0xffffffffu, fi - f, b);
+    if (lane == 0) {
+      s.bucket = c * (SP_BUCKETS / SP_COARSE) + b;
+      s.above = before;
+      s.total = total;
+    }
+  }
+  __syncthreads();
+}
+
+// The entries for which take(l, index) holds, in no order, in block 0's s.ent; their number, the same
+// for all.  Above SP_LIST the list is of no use.
+template <class Take>
+__device__ int gather(cg::cluster_group& cl, SampleShared& s, const Row& row, Take take) {
+  const int tid = threadIdx.x, lane = tid & 31, C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  if (tid == 0) s.n = 0;
+  __syncthreads();
+  for (int j0 = 0; j0 < row.cnt; j0 += SP_THREADS) {
+    const int j = j0 + tid;
+    const float l = j < row.cnt ? row.x[j] : 0.f;
+    const bool in = j < row.cnt && take(l, row.lo + j);
+    const uint32_t m = __ballot_sync(0xffffffffu, in);
+    if (m == 0) continue;
+    int at = 0;
+    if (lane == __ffs(m) - 1) at = atomicAdd(&s.n, __popc(m));
+    at = __shfl_sync(0xffffffffu, at, __ffs(m) - 1) + __popc(m & ((1u << lane) - 1));
+    if (in && at < SP_LIST) s.ent[at] = entry_of(l, row.lo + j);
+  }
+  cl.sync();
+  int n = 0;
+  for (int r = 0; r < C; ++r) {
+    const int c = *cl.map_shared_rank(&s.n, r);
+    if (rank == 0 && r > 0 && n + c <= SP_LIST) {
+      const u64* p = cl.map_shared_rank(s.ent, r);
+      for (int i = tid; i < c; i += SP_THREADS) s.ent[n + i] = p[i];
+    }
+    n += c;
+  }
+  __syncthreads();
+  return n;
+}
+
+// s.ent[0, n) in descending order (bitonic); entries differ from one another.
+__device__ void sort_list(u64* ent, int n, int* padded) {
+  int N = 32;
+  while (N < n) N <<= 1;
+  for (int i = n + threadIdx.x; i < N; i += SP_THREADS) ent[i] = 0;
+  __syncthreads();
+  for (int k = 2; k <= N; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = threadIdx.x; i < N / 2; i += SP_THREADS) {
+        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+        const u64 x = ent[a], y = ent[b];
+        if ((x < y) == ((a & k) == 0)) ent[a] = y, ent[b] = x;
+      }
+      __syncthreads();
+    }
+  *padded = N;
+}
+
+// pre[i] = value(0) + .. + value(i) for i < n <= 2 * SP_THREADS.
+template <class Value>
+__device__ void scan_list(SampleShared& s, int n, Value value) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const u64 a = 2 * tid < n ? value(2 * tid) : 0, b = 2 * tid + 1 < n ? value(2 * tid + 1) : 0;
+  u64 incl = warp_scan64(a + b);
+  if (lane == 31) s.warp64[warp] = incl;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) incl += s.warp64[w];
+  if (2 * tid < n) s.list.pre[2 * tid] = incl - b;
+  if (2 * tid + 1 < n) s.list.pre[2 * tid + 1] = incl;
+  __syncthreads();
+}
+
+// The number of leading list entries whose running sum s.list.pre is below `want`.
+__device__ int count_below(SampleShared& s, int n, u64 want) {
+  const int tid = threadIdx.x;
+  return __syncthreads_count(2 * tid < n && s.list.pre[2 * tid] < want) +
+         __syncthreads_count(2 * tid + 1 < n && s.list.pre[2 * tid + 1] < want);
+}
+
+// The smallest entry X for which the sum of value(l, index) over the entries >= X reaches `need`, by
+// radix passes over the 56 bits of an entry; for any number of entries and equal logits.
+template <class Value>
+__device__ u64 radix_border(cg::cluster_group& cl, SampleShared& s, const Row& row, u64 need, Value value) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = (int)cl.num_blocks();
+  u64 prefix = 0;
+  for (int shift = 48, p = 0; shift >= 0; shift -= 8, ++p) {
+    uint32_t *lo = s.hist.lo + (p & 1) * 256, *hi = s.hist.hi + (p & 1) * 256;
+    cl.sync();  // the pass before last is read by all
+    if (tid < 256) lo[tid] = hi[tid] = 0;
+    __syncthreads();
+    for (int j = tid; j < row.cnt; j += SP_THREADS) {
+      const float l = row.x[j];
+      const u64 e = entry_of(l, row.lo + j);
+      if (((e ^ prefix) >> 8) >> shift) continue;
+      const u64 v = value(l, row.lo + j);
+      if (v) add64(&lo[(e >> shift) & 255], &hi[(e >> shift) & 255], v);
     }
     cl.sync();
-    if (tid < 256) {
-      u64 t = 0;
-      for (int r = 0; r < C; ++r) t += cl.map_shared_rank(h, r)[tid];
-      s.tot[tid] = t;
-    }
-    __syncthreads();
-    if (warp == 0) {
+    if (warp == 0) {  // the digit at which the sum from above reaches `need`
       u64 v[8], sum = 0;
-      for (int e = 0; e < 8; ++e) sum += v[e] = s.tot[255 - (lane * 8 + e)];
-      u64 incl = sum;
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = 0;
+        for (int r = 0; r < C; ++r)
+          v[e] += (u64)cl.map_shared_rank(hi, r)[255 - lane * 8 - e] << 32 | cl.map_shared_rank(lo, r)[255 - lane * 8 - e];
+        sum += v[e];
       }
+      const u64 incl = warp_scan64(sum);
+      const uint32_t hit = __ballot_sync(0xffffffffu, incl >= need);
       u64 above = incl - sum;
-      if (above < need && incl >= need) {
-        int e = 0;
-        while (above + v[e] < need) above += v[e++];
-        s.prefix = prefix | ((uint32_t)(255 - (lane * 8 + e)) << shift);
-        s.left = need - above;
+      if (lane == __ffs(hit) - 1) {
+        int d = 0;
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (!done && above + v[e] < need) above += v[e], ++d;
+          else done = true;
+        }
+        s.border = prefix | (u64)(255 - lane * 8 - d) << shift;
+        s.above = above;
       }
     }
     __syncthreads();
-    prefix = s.prefix;
-    need = s.left;
+    prefix = s.border;
+    need -= s.above;
   }
-  *left = need;
+  cl.sync();  // the last pass is read by all
   return prefix;
 }
 
-__global__ void __launch_bounds__(SP_THREADS) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) float x[];
   __shared__ SampleShared s;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  const int row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const float* src = a.logits + (size_t)row * a.ld;
-  const int lo = min(a.vocab, rank * a.slice), cnt = min(a.vocab, lo + a.slice) - lo;
+  const int r = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  Row row;
+  row.x = x;
+  row.lo = min(a.vocab, rank * a.slice);
+  row.cnt = min(a.vocab, row.lo + a.slice) - row.lo;
+  row.tab = s.tab;
+  const float* src = a.logits + (size_t)r * a.ld + row.lo;
+  const float temp = a.temperature ? a.temperature[r] : 1.f, p = a.top_p ? a.top_p[r] : 1.f;
+  const float mp = a.min_p ? a.min_p[r] : 0.f, uf = a.u[r];
+  int k = a.top_k ? a.top_k[r] : 0;
 
-  float m = -INFINITY;
-  int bad = 0;
-  for (int j = tid; j < cnt; j += SP_THREADS) {
-    const float l = __ldg(src + lo + j);
+  // the row, its largest and its smallest finite logit, and whether it holds a NaN
+  float hi = -INFINITY, lo = INFINITY;
+  bool bad = false;
+#pragma unroll 8
+  for (int j = tid; j < row.cnt; j += SP_THREADS) {
+    const float l = __ldcs(src + j);
     x[j] = l;
-    m = fmaxf(m, l);
+    hi = fmaxf(hi, l);
+    if (l > -INFINITY) lo = fminf(lo, l);
     bad |= l != l;
   }
-  m = warp_max(m);
-  bad = __any_sync(0xffffffffu, bad);
-  if (lane == 0) {
-    s.warp32[warp] = __float_as_uint(m);
-    if (warp == 0) s.bad = 0;
-  }
-  __syncthreads();
-  if (lane == 0 && bad) s.bad = 1;
-  if (tid == 0) {
-    for (int w = 1; w < SP_THREADS / 32; ++w) m = fmaxf(m, __uint_as_float(s.warp32[w]));
-    s.fmax = m;
+  if (tid < 64) s.tab[tid] = exp2((double)tid / 64);
+  hi = warp_max(hi);
+  lo = -warp_max(-lo);
+  if (lane == 0) s.warp64[warp] = (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo);
+  bad = __syncthreads_or(bad);
+  if (tid < 32) {
+    const u64 v = s.warp64[lane % SP_WARPS];
+    hi = warp_max(__uint_as_float((uint32_t)(v >> 32)));
+    lo = -warp_max(-__uint_as_float((uint32_t)v));
+    if (tid == 0) s.fmax = hi, s.fmin = lo, s.bad = bad;
   }
   cl.sync();
-  float lmax = -INFINITY;
-  bad = 0;
-  for (int r = 0; r < C; ++r) {
-    lmax = fmaxf(lmax, *cl.map_shared_rank(&s.fmax, r));
-    bad |= *cl.map_shared_rank(&s.bad, r);
+  {
+    const int q = lane < C ? lane : 0;  // a block of the cluster to each lane
+    hi = warp_max(*cl.map_shared_rank(&s.fmax, q));
+    lo = -warp_max(-*cl.map_shared_rank(&s.fmin, q));
+    bad = __any_sync(0xffffffffu, *cl.map_shared_rank(&s.bad, q));
   }
-  const float temp = a.temperature ? a.temperature[row] : 1.f;
-  const bool greedy = temp == 0.f;
-  const bool none = bad || lmax == -INFINITY || !(temp >= 0.f);
-  if (none) {  // the same for the whole cluster
+  row.lmax = hi;
+  row.lmax_d = (double)hi;
+  const bool greedy = temp == 0.f, ok = temp >= 0.f;
+  if (bad || !ok || hi == -INFINITY) {  // the same for the whole cluster
     if (rank == 0 && tid == 0) {
-      a.ids[row] = -1;
-      if (a.logprob) a.logprob[row] = bad || !(temp >= 0.f) ? NAN : -INFINITY;
+      a.ids[r] = -1;
+      if (a.logprob) a.logprob[r] = bad || !ok ? NAN : -INFINITY;
     }
-    cl.sync();  // fmax and bad are read by the other blocks
+    cl.sync();  // the other blocks have read fmax and bad
     return;
   }
-  const double T = greedy ? 1.0 : (double)temp;
-  int k = a.top_k ? a.top_k[row] : 0;
+  row.inv_t = greedy ? 1.0 : 1.0 / (double)temp;
   if (greedy) k = 1;
-  uint32_t Tk = 0, ties = 0xffffffffu;  // tokens with key > Tk stay, and the first `ties` of key Tk
-  if (k > 0 && k < a.vocab) {
-    u64 left;
-    Tk = radix_find(cl, s, x, cnt, (u64)k, &left, [](float, uint32_t) { return (u64)1; });
-    ties = (uint32_t)left;
-  }
-  const float p = a.top_p ? a.top_p[row] : 1.f;
-  if (p < 1.f) {
-    const u64 wt = ties == 0xffffffffu ? 0 : weight_of(logit_of(Tk), lmax, T);
-    u64 mass = 0;
-    for (int j = tid; j < cnt; j += SP_THREADS)
-      if (key_of(x[j]) > Tk || ties == 0xffffffffu) mass += weight_of(x[j], lmax, T);
-    mass = block_sum64(mass, s.warp64);
-    if (tid == 0) s.part64[0] = mass;
-    cl.sync();
-    mass = ties == 0xffffffffu ? 0 : ties * wt;
-    for (int r = 0; r < C; ++r) mass += *cl.map_shared_rank(&s.part64[0], r);
-    const double want = ceil((double)p * (double)mass);
-    const u64 need = want < 1.0 ? 1 : (u64)want;
-    const uint32_t Tk0 = Tk, ties0 = ties;
-    const u64 above = mass - (ties0 == 0xffffffffu ? 0 : ties0 * wt);
-    if (ties0 == 0xffffffffu || need <= above) {
-      u64 left;
-      Tk = radix_find(cl, s, x, cnt, need, &left, [&](float l, uint32_t key) {
-        return key > Tk0 || ties0 == 0xffffffffu ? weight_of(l, lmax, T) : (u64)0;
-      });
-      const u64 w = weight_of(logit_of(Tk), lmax, T);
-      ties = (uint32_t)((left + w - 1) / w);
-    } else {
-      ties = (uint32_t)((need - above + wt - 1) / wt);
-    }
-  }
-  double least = a.min_p ? fmin((double)a.min_p[row], 1.0) * SP_ONE : 0.0;
-  if (!(least >= 0.0)) least = 0.0;
-
-  // which tokens of key Tk stay: the first `ties` in index order
-  uint32_t eq_base = 0;
-  if (ties != 0xffffffffu) {
-    uint32_t c = 0;
-    for (int j = tid; j < cnt; j += SP_THREADS) c += key_of(x[j]) == Tk;
-    const u64 t = block_sum64(c, s.warp64);
-    if (tid == 0) s.part32[0] = (uint32_t)t;
-    cl.sync();
-    for (int r = 0; r < rank; ++r) eq_base += *cl.map_shared_rank(&s.part32[0], r);
-  }
-  // weight of every staying token, chunk by chunk in index order; the sum of this block
-  auto chunk_weight = [&](int j0, uint32_t& base) {
-    const int j = j0 + tid;
-    const bool in = j < cnt;
-    const float l = in ? x[j] : -INFINITY;
-    const uint32_t key = key_of(l);
-    bool stays = in;
-    if (ties != 0xffffffffu) {
-      const uint32_t eq = __ballot_sync(0xffffffffu, in && key == Tk);
-      __syncthreads();
-      if (lane == 0) s.warp32[warp] = __popc(eq);
-      __syncthreads();
-      uint32_t before = 0, all = 0;
-      for (int w = 0; w < 32; ++w) {
-        if (w < warp) before += s.warp32[w];
-        all += s.warp32[w];
-      }
-      stays = in && (key > Tk || (key == Tk && base + before + __popc(eq & ((1u << lane) - 1)) < ties));
-      base += all;
-    }
-    if (!stays) return (u64)0;
-    const u64 w = weight_of(l, lmax, T);
-    return (double)w >= least ? w : (u64)0;
-  };
-  u64 sum = 0;
-  uint32_t base = eq_base;
-  for (int j0 = 0; j0 < cnt; j0 += SP_THREADS) sum += chunk_weight(j0, base);
-  sum = block_sum64(sum, s.warp64);
-  if (tid == 0) s.part64[1] = sum;
-  cl.sync();
-  u64 total = 0, before = 0;
-  for (int r = 0; r < C; ++r) {
-    const u64 t = *cl.map_shared_rank(&s.part64[1], r);
-    if (r < rank) before += t;
-    total += t;
-  }
-  const float uf = a.u[row];
+  if (k >= a.vocab) k = 0;
+  const u64 least = mp > 0.f ? (u64)ceil(fmin((double)mp, 1.0) * SP_ONE) : 0;
   const double ud = uf > 0.f ? (double)uf : 0.0;
-  const double at_d = floor(ud * (double)total);
-  const u64 at = at_d >= (double)total ? total - 1 : (u64)at_d < total ? (u64)at_d : total - 1;
-  if (before <= at && at < before + sum) {  // this block holds the token
-    base = eq_base;
-    u64 run = before;
-    for (int j0 = 0; j0 < cnt; j0 += SP_THREADS) {
-      const u64 w = chunk_weight(j0, base);
-      u64 incl = w;
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
+  auto drawn = [&](u64 total) {  // the weight that the running sum has to exceed
+    const double at = floor(ud * (double)total);
+    return at >= (double)total || (u64)at >= total ? total - 1 : (u64)at;
+  };
+  auto need_of = [&](u64 total) {  // top-p: the weight that stays
+    const double want = ceil((double)p * (double)total);
+    return want < 1.0 ? 1ull : (u64)want;
+  };
+
+  u64 border = 0;  // entries >= border stay
+  if (k > 0) {
+    Buckets bucket = {hi, 0.f};
+    const float range = fminf(hi - lo, 64.f * fmaxf(1.f, greedy ? 1.f : temp));
+    bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
+    find_bucket(cl, s, row, bucket, false, [](float, int) { return (u64)1; },
+                [&](u64 total) { return total < (u64)k ? total : (u64)k; });
+    const int last = s.bucket;
+    const u64 want = s.total < (u64)k ? s.total : (u64)k;  // tokens of -infinity never stay
+    const int n = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket(l) <= last; });
+    if (n <= SP_LIST) {  // all on the sorted list, by one block
+      if (rank == 0) {
+        int N;
+        sort_list(s.ent, n, &N);
+        int m = (int)want;
+        for (int i = tid; i < m; i += SP_THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
+        __syncthreads();
+        scan_list(s, m, [&](int i) { return s.list.wt[i]; });
+        if (p < 1.f) m = count_below(s, m, need_of(s.list.pre[m - 1])) + 1;
+        if (least)  // weights descend
+          m = __syncthreads_count(2 * tid < m && s.list.wt[2 * tid] >= least) +
+              __syncthreads_count(2 * tid + 1 < m && s.list.wt[2 * tid + 1] >= least);
+        const u64 total = s.list.pre[m - 1], at = drawn(total);
+        __syncthreads();
+        // index order: entries become (index, place), inverted since the sort descends
+        for (int i = tid; i < m; i += SP_THREADS) s.ent[i] = ~((u64)index_of(s.ent[i]) << 32 | (uint32_t)i);
+        sort_list(s.ent, m, &N);
+        scan_list(s, m, [&](int i) { return s.list.wt[(uint32_t)~s.ent[i]]; });
+        const int place = count_below(s, m, at + 1);
+        if (tid == 0) {
+          const u64 e = ~s.ent[place];
+          a.ids[r] = (int)(e >> 32);
+          if (a.logprob) a.logprob[r] = (float)log((double)s.list.wt[(uint32_t)e] / (double)total);
+        }
       }
-      __syncthreads();
-      if (lane == 31) s.warp64[warp] = incl;
-      __syncthreads();
-      u64 wb = run, all = 0;
-      for (int q = 0; q < 32; ++q) {
-        if (q < warp) wb += s.warp64[q];
-        all += s.warp64[q];
+      cl.sync();  // block 0 has read the others' entries
+      return;
+    }
+    cl.sync();  // the counts are read by all
+    const int in_last = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket(l) == last; });
+    if (in_last <= SP_LIST) {
+      if (rank == 0) {
+        int N;
+        sort_list(s.ent, in_last, &N);
+        if (tid == 0) s.border = s.ent[(int)(want - s.above) - 1];
       }
-      if (wb + incl - w <= at && at < wb + incl) {
-        a.ids[row] = lo + j0 + tid;
-        if (a.logprob) a.logprob[row] = (float)log((double)w / (double)total);
-      }
-      run += all;
-      if (run > at) break;
+      cl.sync();
+      border = *cl.map_shared_rank(&s.border, 0);
+      cl.sync();
+    } else {
+      border = radix_border(cl, s, row, want, [](float l, int) { return (u64)(l > -INFINITY); });
     }
   }
-  cl.sync();  // part64 is read by the other blocks
+  if (p < 1.f) {
+    const u64 first = border;
+    Buckets bucket = {hi, 0.f};
+    const float range = fminf(hi - lo, (float)(31.5 / row.inv_t));
+    bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
+    auto weight = [&](float l, int i) { return first == 0 || entry_of(l, i) >= first ? row.weight(l) : (u64)0; };
+    find_bucket(cl, s, row, bucket, true, weight, need_of);
+    const int last = s.bucket;
+    const u64 want = need_of(s.total), above = s.above;
+    const int n = gather(cl, s, row, [&](float l, int i) {
+      return bucket(l) == last && (first == 0 || entry_of(l, i) >= first);
+    });
+    if (n <= SP_LIST) {
+      if (rank == 0) {
+        int N;
+        sort_list(s.ent, n, &N);
+        for (int i = tid; i < n; i += SP_THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
+        __syncthreads();
+        scan_list(s, n, [&](int i) { return s.list.wt[i]; });
+        const int place = count_below(s, n, want - above);
+        if (tid == 0) s.border = s.ent[place];
+      }
+      cl.sync();
+      border = *cl.map_shared_rank(&s.border, 0);
+      cl.sync();
+    } else {
+      border = radix_border(cl, s, row, want, weight);
+    }
+  }
+
+  // the sums of each warp's part of this block's logits, then the warp that holds the token
+  const float edge = border ? logit_of(border) : -INFINITY;
+  const int edge_index = border ? index_of(border) : a.vocab;
+  auto staying = [&](int j) {
+    const float l = x[j];
+    if (!(l > edge || (l == edge && row.lo + j <= edge_index))) return (u64)0;
+    const u64 w = row.weight(l);
+    return w >= least ? w : (u64)0;
+  };
+  const int part = (row.cnt + SP_WARPS * 32 - 1) / (SP_WARPS * 32) * 32;
+  const int w0 = min(row.cnt, warp * part), w1 = min(row.cnt, w0 + part);
+  u64 sum = 0;
+  for (int j = w0 + lane; j < w1; j += 32) sum += staying(j);
+  sum = warp_sum64(sum);
+  if (lane == 0) s.warp64[warp] = sum;
+  __syncthreads();
+  u64 before = 0;
+  {
+    const u64 v = lane < SP_WARPS ? s.warp64[lane] : 0;
+    const u64 incl = warp_scan64(v);
+    before = __shfl_sync(0xffffffffu, incl - v, warp);
+    if (tid == 31) s.total = incl;
+  }
+  cl.sync();
+  const u64 block_sum = lane < C ? *cl.map_shared_rank(&s.total, lane) : 0;
+  const u64 block_incl = warp_scan64(block_sum);
+  const u64 total = __shfl_sync(0xffffffffu, block_incl, 31), at = drawn(total);
+  before += __shfl_sync(0xffffffffu, block_incl - block_sum, rank);
+  if (before <= at && at < before + sum) {
+    for (int j0 = w0; j0 < w1; j0 += 32) {
+      const u64 w = j0 + lane < w1 ? staying(j0 + lane) : 0;
+      const u64 incl = before + warp_scan64(w);
+      if (incl - w <= at && at < incl) {
+        a.ids[r] = row.lo + j0 + lane;
+        if (a.logprob) a.logprob[r] = (float)log((double)w / (double)total);
+      }
+      before = __shfl_sync(0xffffffffu, incl, 31);
+      if (before > at) break;
+    }
+  }
+  cl.sync();  // the other blocks have read this one's sum
 }
 
+// Blocks of a row: slices that leave room for two blocks on an SM, and more where there are few rows.
 int cluster_of(int rows, int vocab) {
   int c = 1;
-  while (c < SP_MAX_CLUSTER && (vocab > SP_SLICE * c || (rows * c < 148 && vocab > 4096 * c))) c *= 2;
+  while (c < SP_MAX_CLUSTER && (vocab > 19456 * c || (rows * c < 148 && vocab > 2048 * c))) c *= 2;
   return c;
 }
 
