@@ -75,7 +75,9 @@ struct SampleShared {
     } list;
   };
   u64 ent[SP_LIST];  // gathered entries
-  double tab[64];    // 2^(i / 64)
+  double tab[16];    // 2^(i / 16)
+  float kept[SP_WARPS][64];               // logits whose weights a warp has yet to sum
+  uint32_t part_lo[SP_WARPS], part_hi[SP_WARPS];  // the sum of each warp's part of the row
   u64 coarse[SP_COARSE];
   u64 warp64[SP_WARPS];
   u64 total, above, border;
@@ -88,28 +90,40 @@ struct SampleShared {
 struct Row {
   const float* x;  // this block's logits
   int lo, cnt;     // their first index and number
-  float lmax;
+  float lmax, floor_;
   double lmax_d, inv_t;
   const double* tab;
 
-  // exp by a table of 2^(i/64) and a polynomial of degree 4 (table-driven, after Tang, 1989): off by
-  // less than 2^-43 of itself.  A token at z <= -31.5 has no weight (exp(-31.2) 2^44 = 1/2), nor has
-  // one next to +infinity or -infinity itself, where z is infinite or a NaN.
+  // exp by a table of 2^(i/16) and a polynomial of degree 6 (table-driven, after Tang, 1989): off by
+  // less than 2^-50 of itself.  16 table entries of 8 bytes are all banks of shared memory once: a
+  // warp reads them without conflicts (a table of 64 with degree 4 took longer).  A token at
+  // z <= -31.5 has no weight (exp(-31.2) 2^44 = 1/2), nor has one next to +infinity or -infinity
+  // itself, where z is infinite or a NaN.
+  // floor_: where lmax and the temperature are finite and ordinary, a logit just above which z is
+  // still below -31.5; else -infinity, and the cases are told apart.
   __device__ __forceinline__ u64 weight(float l) const {
-    if (l == lmax) return 1ull << SP_BITS;
-    const double z = ((double)l - lmax_d) * inv_t;
-    if (!(z > -31.5)) return 0;
-    constexpr double kShift = 6755399441055744.0;                   // 1.5 * 2^52: rounds to an integer
-    const double t = fma(z, 92.332482616893656877, kShift);         // 64 / ln 2
+    constexpr double kShift = 6755399441055744.0;  // 1.5 * 2^52: a sum with it is rounded to an integer
+    double z = ((double)fmaxf(l, floor_) - lmax_d) * inv_t;
+    bool some = true;
+    if (floor_ == -INFINITY) {
+      z = l == lmax ? 0.0 : z;
+      some = z > -31.5;
+      z = some ? z : 0.0;
+    }
+    const double t = fma(z, 23.083120654223414215, kShift);     // 16 / ln 2
     const int n = __double2loint(t);
-    const double r = fma(t - kShift, -0.010830424696249145, z);     // ln 2 / 64; |r| <= 0.0055
-    double p = fma(r, 1.0 / 24, 1.0 / 6);
+    const double r = fma(t - kShift, -0.043321698784996581839, z);  // ln 2 / 16; |r| <= 0.0217
+    double p = fma(r, 1.0 / 720, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
-    p *= tab[n & 63];
-    const double s = __hiloint2double(__double2hiint(p) + (((n >> 6) + SP_BITS) << 20), __double2loint(p));
-    return (u64)__double_as_longlong(s + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52: to the nearest integer
+    p *= tab[n & 15];
+    const double s = __hiloint2double(__double2hiint(p) + ((n & ~15) << 16) + (SP_BITS << 20), __double2loint(p));
+    const double w = s + 4503599627370496.0;  // + 2^52: the nearest integer, in the low bits
+    const u64 v = (u64)(__double2hiint(w) & 0xfffff) << 32 | (uint32_t)__double2loint(w);
+    return some ? v : 0;
   }
 };
 
@@ -138,34 +152,40 @@ __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, u64 v) {
 // Equal buckets of lmax - l: at `per` buckets to a unit, the last one holds the rest.
 struct Buckets {
   float lmax, per;
-  __device__ __forceinline__ int operator()(float l) const {
-    return l == lmax ? 0 : (int)fminf((lmax - l) * per, (float)(SP_BUCKETS - 1));
+  __device__ __forceinline__ float place(float l) const {
+    return l == lmax ? 0.f : fminf((lmax - l) * per, (float)(SP_BUCKETS - 1));
   }
+  __device__ __forceinline__ int operator()(float l) const { return (int)place(l); }
 };
 
 // The histogram over the cluster of value(l, index) and the bucket in which the running sum from
 // the largest logit on reaches need(total): s.bucket, s.above (the sum before it), s.total.  Every
 // block finds the same.
-template <class Value, class Need>
-__device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& row, const Buckets& bucket, bool wide,
-                            Value value, Need need) {
+template <bool wide, class Value, class Need>
+__device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& row, const Buckets& bucket, Value value,
+                            Need need) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = (int)cl.num_blocks();
   for (int i = tid; i < SP_BUCKETS; i += SP_THREADS) s.hist.lo[i] = s.hist.hi[i] = 0;
   __syncthreads();
-  if (wide) {
-    for (int j = tid; j < row.cnt; j += SP_THREADS) {
-      const float l = row.x[j];
-      const u64 v = value(l, row.lo + j);
-      if (v) {
-        const int b = bucket(l);
-        add64(&s.hist.lo[b], &s.hist.hi[b], v);
+  constexpr int U = 4;  // logits of a thread whose weights are computed together
+  for (int j0 = tid; j0 < row.cnt; j0 += U * SP_THREADS) {
+    u64 v[U];
+    int at[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = j0 + i * SP_THREADS;
+      const float l = j < row.cnt ? row.x[j] : -INFINITY;
+      v[i] = l > -INFINITY ? value(l, row.lo + j) : 0;
+      at[i] = bucket(l);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (v[i]) {
+        if (wide)
+          add64(&s.hist.lo[at[i]], &s.hist.hi[at[i]], v[i]);
+        else
+          atomicAdd(&s.hist.lo[at[i]], (uint32_t)v[i]);
       }
-    }
-  } else {
-    for (int j = tid; j < row.cnt; j += SP_THREADS) {
-      const float l = row.x[j];
-      if (l != -INFINITY) atomicAdd(&s.hist.lo[bucket(l)], 1u);
-    }
   }
   __syncthreads();
   for (int c = warp; c < SP_COARSE; c += SP_WARPS) {
@@ -205,36 +225,76 @@ __device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& r
   __syncthreads();
 }
 
-// The entries for which take(l, index) holds, in no order, in block 0's s.ent; their number, the same
-// for all.  Above SP_LIST the list is of no use.
-template <class Take>
-__device__ int gather(cg::cluster_group& cl, SampleShared& s, const Row& row, Take take) {
-  const int tid = threadIdx.x, lane = tid & 31, C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  if (tid == 0) s.n = 0;
-  __syncthreads();
-  for (int j0 = 0; j0 < row.cnt; j0 += SP_THREADS) {
-    const int j = j0 + tid;
-    const float l = j < row.cnt ? row.x[j] : 0.f;
-    const bool in = j < row.cnt && take(l, row.lo + j);
-    const uint32_t m = __ballot_sync(0xffffffffu, in);
-    if (m == 0) continue;
-    int at = 0;
-    if (lane == __ffs(m) - 1) at = atomicAdd(&s.n, __popc(m));
-    at = __shfl_sync(0xffffffffu, at, __ffs(m) - 1) + __popc(m & ((1u << lane) - 1));
-    if (in && at < SP_LIST) s.ent[at] = entry_of(l, row.lo + j);
-  }
+// A warp's lanes for which `in` holds put their entries behind this block's others.
+__device__ __forceinline__ void append(SampleShared& s, bool in, float l, int index) {
+  const uint32_t m = __ballot_sync(0xffffffffu, in);
+  if (m == 0) return;
+  const int lane = threadIdx.x & 31;
+  int at = 0;
+  if (lane == __ffs(m) - 1) at = atomicAdd(&s.n, __popc(m));
+  at = __shfl_sync(0xffffffffu, at, __ffs(m) - 1) + __popc(m & ((1u << lane) - 1));
+  if (in && at < SP_LIST) s.ent[at] = entry_of(l, index);
+}
+
+// The blocks' entries, in no order, in block 0's s.ent; their number, the same for all.  Above
+// SP_LIST the list is of no use.
+__device__ int collect(cg::cluster_group& cl, SampleShared& s) {
+  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   cl.sync();
   int n = 0;
   for (int r = 0; r < C; ++r) {
     const int c = *cl.map_shared_rank(&s.n, r);
     if (rank == 0 && r > 0 && n + c <= SP_LIST) {
       const u64* p = cl.map_shared_rank(s.ent, r);
-      for (int i = tid; i < c; i += SP_THREADS) s.ent[n + i] = p[i];
+      for (int i = threadIdx.x; i < c; i += SP_THREADS) s.ent[n + i] = p[i];
     }
     n += c;
   }
   __syncthreads();
   return n;
+}
+
+template <class Take>
+__device__ int gather(cg::cluster_group& cl, SampleShared& s, const Row& row, Take take) {
+  if (threadIdx.x == 0) s.n = 0;
+  __syncthreads();
+  for (int j0 = 0; j0 < row.cnt; j0 += SP_THREADS) {
+    const int j = j0 + threadIdx.x;
+    const float l = j < row.cnt ? row.x[j] : -INFINITY;
+    append(s, j < row.cnt && take(l, row.lo + j), l, row.lo + j);
+  }
+  return collect(cl, s);
+}
+
+// The sum of the weights, where at least `least`, of the logits j in [j0, j1) for which keep(l, j)
+// holds, by one warp.  The few that are kept are first put side by side, 32 for each exponential.
+template <class Keep>
+__device__ u64 sum_kept(SampleShared& s, const Row& row, int j0, int j1, u64 least, Keep keep) {
+  const int lane = threadIdx.x & 31;
+  float* buf = s.kept[threadIdx.x >> 5];
+  int n = 0;
+  u64 sum = 0;
+  auto add = [&](bool in, float l) {
+    const u64 w = in ? row.weight(l) : 0;
+    if (w >= least) sum += w;
+  };
+  for (int j = j0 + lane; j - lane < j1; j += 32) {
+    const float l = j < j1 ? row.x[j] : -INFINITY;
+    const bool in = keep(l, j) && j < j1;
+    const uint32_t m = __ballot_sync(0xffffffffu, in);
+    if (in) buf[n + __popc(m & ((1u << lane) - 1))] = l;
+    n += __popc(m);
+    if (n >= 32) {
+      n -= 32;
+      __syncwarp();
+      add(true, buf[n + lane]);
+      __syncwarp();
+    }
+  }
+  __syncwarp();
+  add(lane < n, buf[lane]);
+  __syncwarp();
+  return warp_sum64(sum);
 }
 
 // s.ent[0, n) in descending order (bitonic); entries differ from one another.
@@ -354,7 +414,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     if (l > -INFINITY) lo = fminf(lo, l);
     bad |= l != l;
   }
-  if (tid < 64) s.tab[tid] = exp2((double)tid / 64);
+  if (tid < 16) s.tab[tid] = exp2((double)tid / 16);
   hi = warp_max(hi);
   lo = -warp_max(-lo);
   if (lane == 0) s.warp64[warp] = (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo);
@@ -384,6 +444,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     return;
   }
   row.inv_t = greedy ? 1.0 : 1.0 / (double)temp;
+  row.floor_ = -INFINITY;
+  if (hi < INFINITY && row.inv_t > 1e-30 && row.inv_t < 1e30) {
+    const float f = (float)(row.lmax_d - 32.0 / row.inv_t);  // z of it lies below -31.5 if hi - f is 32 T, to a rounding
+    if (f > -INFINITY && ((double)f - row.lmax_d) * row.inv_t < -31.5) row.floor_ = f;
+  }
   if (greedy) k = 1;
   if (k >= a.vocab) k = 0;
   const u64 least = mp > 0.f ? (u64)ceil(fmin((double)mp, 1.0) * SP_ONE) : 0;
@@ -402,7 +467,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     Buckets bucket = {hi, 0.f};
     const float range = fminf(hi - lo, 64.f * fmaxf(1.f, greedy ? 1.f : temp));
     bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
-    find_bucket(cl, s, row, bucket, false, [](float, int) { return (u64)1; },
+    find_bucket<false>(cl, s, row, bucket, [](float, int) { return (u64)1; },
                 [&](u64 total) { return total < (u64)k ? total : (u64)k; });
     const int last = s.bucket;
     const u64 want = s.total < (u64)k ? s.total : (u64)k;  // tokens of -infinity never stay
@@ -450,18 +515,35 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
       border = radix_border(cl, s, row, want, [](float l, int) { return (u64)(l > -INFINITY); });
     }
   }
+  // each warp has a part of this block's logits; what min-p lets go of for certain needs no weight
+  const int part = max(32, (row.cnt + SP_WARPS * 32 - 1) / (SP_WARPS * 32) * 32);
+  const int w0 = min(row.cnt, warp * part), w1 = min(row.cnt, w0 + part);
+  const float cut = least ? (float)(row.lmax_d + (log(fmin((double)mp, 1.0)) - 1e-3) / row.inv_t) : -INFINITY;
+  const float low = cut > -INFINITY ? nextafterf(cut, -INFINITY) : -INFINITY;  // (NaN and +infinity: no cut below)
+  bool summed = false;
   if (p < 1.f) {
     const u64 first = border;
     Buckets bucket = {hi, 0.f};
     const float range = fminf(hi - lo, (float)(31.5 / row.inv_t));
     bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
-    auto weight = [&](float l, int i) { return first == 0 || entry_of(l, i) >= first ? row.weight(l) : (u64)0; };
-    find_bucket(cl, s, row, bucket, true, weight, need_of);
-    const int last = s.bucket;
+    auto weight = [&](float l, int i) { return entry_of(l, i) >= first ? row.weight(l) : (u64)0; };
+    if (first == 0)
+      find_bucket<true>(cl, s, row, bucket, [&](float l, int) { return row.weight(l); }, need_of);
+    else
+      find_bucket<true>(cl, s, row, bucket, weight, need_of);
+    const float last = (float)s.bucket;
     const u64 want = need_of(s.total), above = s.above;
-    const int n = gather(cl, s, row, [&](float l, int i) {
-      return bucket(l) == last && (first == 0 || entry_of(l, i) >= first);
+    // before the border's bucket all stay; the bucket's own go on the list
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    const u64 sure = sum_kept(s, row, w0, w1, least, [&](float l, int j) {
+      const float at = bucket.place(l);
+      const bool in = j < w1 && (first == 0 || entry_of(l, row.lo + j) >= first);
+      append(s, in && at >= last && at < last + 1.f, l, row.lo + j);
+      return in && at < last && l >= low;
     });
+    if (lane == 0) s.part_lo[warp] = (uint32_t)sure, s.part_hi[warp] = (uint32_t)(sure >> 32);
+    const int n = collect(cl, s);
     if (n <= SP_LIST) {
       if (rank == 0) {
         int N;
@@ -474,26 +556,34 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
       }
       cl.sync();
       border = *cl.map_shared_rank(&s.border, 0);
-      cl.sync();
+      // those of the list that stay and lie in this block join their warp's sum
+      const int own = rank == 0 ? n : s.n;
+      for (int i = tid; i < own; i += SP_THREADS) {
+        const u64 e = s.ent[i];
+        const int j = index_of(e) - row.lo;
+        if (e < border || j < 0 || j >= row.cnt) continue;
+        const u64 w = row.weight(logit_of(e));
+        if (w && w >= least) add64(&s.part_lo[j / part], &s.part_hi[j / part], w);
+      }
+      summed = true;
+      __syncthreads();
     } else {
       border = radix_border(cl, s, row, want, weight);
     }
   }
 
-  // the sums of each warp's part of this block's logits, then the warp that holds the token
+  // the sums of the warps' parts, then the warp that holds the token walks its part
   const float edge = border ? logit_of(border) : -INFINITY;
   const int edge_index = border ? index_of(border) : a.vocab;
-  auto staying = [&](int j) {
-    const float l = x[j];
-    if (!(l > edge || (l == edge && row.lo + j <= edge_index))) return (u64)0;
-    const u64 w = row.weight(l);
-    return w >= least ? w : (u64)0;
+  auto stays = [&](float l, int j) {
+    return (l > edge || (l == edge && row.lo + j <= edge_index)) && l >= low;
   };
-  const int part = (row.cnt + SP_WARPS * 32 - 1) / (SP_WARPS * 32) * 32;
-  const int w0 = min(row.cnt, warp * part), w1 = min(row.cnt, w0 + part);
-  u64 sum = 0;
-  for (int j = w0 + lane; j < w1; j += 32) sum += staying(j);
-  sum = warp_sum64(sum);
+  u64 sum;
+  if (summed) {
+    sum = (u64)s.part_hi[warp] << 32 | s.part_lo[warp];
+  } else {
+    sum = sum_kept(s, row, w0, w1, least, stays);
+  }
   if (lane == 0) s.warp64[warp] = sum;
   __syncthreads();
   u64 before = 0;
@@ -508,16 +598,32 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   const u64 block_incl = warp_scan64(block_sum);
   const u64 total = __shfl_sync(0xffffffffu, block_incl, 31), at = drawn(total);
   before += __shfl_sync(0xffffffffu, block_incl - block_sum, rank);
-  if (before <= at && at < before + sum) {
-    for (int j0 = w0; j0 < w1; j0 += 32) {
-      const u64 w = j0 + lane < w1 ? staying(j0 + lane) : 0;
-      const u64 incl = before + warp_scan64(w);
+  if (tid == 0) s.n = -1;
+  __syncthreads();
+  if (lane == 0 && before <= at && at < before + sum) {
+    s.n = warp;
+    s.above = before;
+  }
+  __syncthreads();
+  if (s.n >= 0) {  // one block of the cluster: all its warps walk the part of that warp
+    u64 run = s.above;
+    const int j0 = s.n * part, j1 = min(row.cnt, j0 + part);
+    for (int j = j0 + tid; j - tid < j1; j += SP_THREADS) {
+      u64 w = j < j1 && stays(x[j], j) ? row.weight(x[j]) : 0;
+      if (w < least) w = 0;
+      u64 incl = warp_scan64(w);
+      __syncthreads();  // warp64 of the round before is read
+      if (lane == 31) s.warp64[warp] = incl;
+      __syncthreads();
+      for (int q = 0; q < SP_WARPS; ++q) {
+        if (q == warp) incl += run;
+        run += s.warp64[q];
+      }
       if (incl - w <= at && at < incl) {
-        a.ids[r] = row.lo + j0 + lane;
+        a.ids[r] = row.lo + j;
         if (a.logprob) a.logprob[r] = (float)log((double)w / (double)total);
       }
-      before = __shfl_sync(0xffffffffu, incl, 31);
-      if (before > at) break;
+      if (run > at) break;
     }
   }
   cl.sync();  // the other blocks have read this one's sum
