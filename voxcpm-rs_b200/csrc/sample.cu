@@ -99,18 +99,16 @@ struct Row {
   // warp reads them without conflicts (a table of 64 with degree 4 took longer).  A token at
   // z <= -31.5 has no weight (exp(-31.2) 2^44 = 1/2), nor has one next to +infinity or -infinity
   // itself, where z is infinite or a NaN.
-  // floor_: where lmax and the temperature are finite and ordinary, a logit just above which z is
-  // still below -31.5; else -infinity, and the cases are told apart.
+  // floor_: where lmax and the temperature are finite and ordinary, a logit at which z is below
+  // -31.5, so that none from there down has a weight; else -infinity, and the cases are told apart.
   __device__ __forceinline__ u64 weight(float l) const {
-    constexpr double kShift = 6755399441055744.0;  // 1.5 * 2^52: a sum with it is rounded to an integer
-    double z = ((double)fmaxf(l, floor_) - lmax_d) * inv_t;
-    bool some = true;
-    if (floor_ == -INFINITY) {
-      z = l == lmax ? 0.0 : z;
-      some = z > -31.5;
-      z = some ? z : 0.0;
-    }
-    const double t = fma(z, 23.083120654223414215, kShift);     // 16 / ln 2
+    if (floor_ > -INFINITY) return l > floor_ ? exp_of(((double)l - lmax_d) * inv_t) : 0;
+    const double z = l == lmax ? 0.0 : ((double)l - lmax_d) * inv_t;
+    return z > -31.5 ? exp_of(z) : 0;
+  }
+  __device__ __forceinline__ u64 exp_of(double z) const {
+    constexpr double kShift = 6755399441055744.0;                   // 1.5 * 2^52: a sum with it is rounded to an integer
+    const double t = fma(z, 23.083120654223414215, kShift);         // 16 / ln 2
     const int n = __double2loint(t);
     const double r = fma(t - kShift, -0.043321698784996581839, z);  // ln 2 / 16; |r| <= 0.0217
     double p = fma(r, 1.0 / 720, 1.0 / 120);
@@ -122,8 +120,7 @@ struct Row {
     p *= tab[n & 15];
     const double s = __hiloint2double(__double2hiint(p) + ((n & ~15) << 16) + (SP_BITS << 20), __double2loint(p));
     const double w = s + 4503599627370496.0;  // + 2^52: the nearest integer, in the low bits
-    const u64 v = (u64)(__double2hiint(w) & 0xfffff) << 32 | (uint32_t)__double2loint(w);
-    return some ? v : 0;
+    return (u64)(__double2hiint(w) & 0xfffff) << 32 | (uint32_t)__double2loint(w);
   }
 };
 
@@ -162,13 +159,30 @@ struct Buckets {
 // the largest logit on reaches need(total): s.bucket, s.above (the sum before it), s.total.  Every
 // block finds the same.
 template <bool wide, class Value, class Need>
-__device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& row, const Buckets& bucket, Value value,
-                            Need need) {
+__device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& row, const Buckets& bucket, bool plain,
+                            Value value, Need need) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = (int)cl.num_blocks();
   for (int i = tid; i < SP_BUCKETS; i += SP_THREADS) s.hist.lo[i] = s.hist.hi[i] = 0;
   __syncthreads();
   constexpr int U = 4;  // logits of a thread whose weights are computed together
-  for (int j0 = tid; j0 < row.cnt; j0 += U * SP_THREADS) {
+  int j0 = tid;
+  if (plain) {  // `per` is finite and no logit above the floor lies behind the last bucket
+    for (; j0 - tid + U * SP_THREADS <= row.cnt; j0 += U * SP_THREADS) {
+      float l[U];
+      u64 v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) l[i] = row.x[j0 + i * SP_THREADS];
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[i] = row.exp_of(((double)fmaxf(l[i], row.floor_) - row.lmax_d) * row.inv_t);
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (l[i] > row.floor_) {
+          const int b = (int)((bucket.lmax - l[i]) * bucket.per);
+          add64(&s.hist.lo[b], &s.hist.hi[b], v[i]);
+        }
+    }
+  }
+  for (; j0 < row.cnt; j0 += U * SP_THREADS) {
     u64 v[U];
     int at[U];
 #pragma unroll
@@ -297,22 +311,31 @@ __device__ u64 sum_kept(SampleShared& s, const Row& row, int j0, int j1, u64 lea
   return warp_sum64(sum);
 }
 
-// s.ent[0, n) in descending order (bitonic); entries differ from one another.
-__device__ void sort_list(u64* ent, int n, int* padded) {
+// ent[0, n) in descending order (bitonic); entries differ from one another.  A thread has one pair
+// of each step; pairs up to 32 apart stay within the 64 entries of a warp, which then needs no
+// barrier with the others.
+__device__ void sort_list(u64* ent, int n) {
   int N = 32;
   while (N < n) N <<= 1;
   for (int i = n + threadIdx.x; i < N; i += SP_THREADS) ent[i] = 0;
   __syncthreads();
-  for (int k = 2; k <= N; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < N / 2; i += SP_THREADS) {
-        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
-        const u64 x = ent[a], y = ent[b];
-        if ((x < y) == ((a & k) == 0)) ent[a] = y, ent[b] = x;
+  static_assert(SP_LIST / 2 <= SP_THREADS, "a pair for each thread");
+  const int i = threadIdx.x;
+  if (i < (N / 2 + 31) / 32 * 32 || N > 64) {  // whole warps; all of them where they meet at barriers
+    for (int k = 2; k <= N; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        if (i < N / 2) {
+          const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+          const u64 x = ent[a], y = ent[b];
+          if ((x < y) == ((a & k) == 0)) ent[a] = y, ent[b] = x;
+        }
+        if (j > 32 || (j == 1 && k > 32 && k < N))  // the step was or the next will be across warps
+          __syncthreads();
+        else
+          __syncwarp();
       }
-      __syncthreads();
-    }
-  *padded = N;
+  }
+  __syncthreads();
 }
 
 // pre[i] = value(0) + .. + value(i) for i < n <= 2 * SP_THREADS.
@@ -467,15 +490,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     Buckets bucket = {hi, 0.f};
     const float range = fminf(hi - lo, 64.f * fmaxf(1.f, greedy ? 1.f : temp));
     bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
-    find_bucket<false>(cl, s, row, bucket, [](float, int) { return (u64)1; },
+    find_bucket<false>(cl, s, row, bucket, false, [](float, int) { return (u64)1; },
                 [&](u64 total) { return total < (u64)k ? total : (u64)k; });
     const int last = s.bucket;
     const u64 want = s.total < (u64)k ? s.total : (u64)k;  // tokens of -infinity never stay
     const int n = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket(l) <= last; });
     if (n <= SP_LIST) {  // all on the sorted list, by one block
       if (rank == 0) {
-        int N;
-        sort_list(s.ent, n, &N);
+        sort_list(s.ent, n);
         int m = (int)want;
         for (int i = tid; i < m; i += SP_THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
         __syncthreads();
@@ -488,7 +510,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
         __syncthreads();
         // index order: entries become (index, place), inverted since the sort descends
         for (int i = tid; i < m; i += SP_THREADS) s.ent[i] = ~((u64)index_of(s.ent[i]) << 32 | (uint32_t)i);
-        sort_list(s.ent, m, &N);
+        sort_list(s.ent, m);
         scan_list(s, m, [&](int i) { return s.list.wt[(uint32_t)~s.ent[i]]; });
         const int place = count_below(s, m, at + 1);
         if (tid == 0) {
@@ -504,8 +526,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     const int in_last = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket(l) == last; });
     if (in_last <= SP_LIST) {
       if (rank == 0) {
-        int N;
-        sort_list(s.ent, in_last, &N);
+        sort_list(s.ent, in_last);
         if (tid == 0) s.border = s.ent[(int)(want - s.above) - 1];
       }
       cl.sync();
@@ -524,30 +545,35 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   if (p < 1.f) {
     const u64 first = border;
     Buckets bucket = {hi, 0.f};
-    const float range = fminf(hi - lo, (float)(31.5 / row.inv_t));
+    const float range = fminf(hi - lo, (float)(32.1 / row.inv_t));  // beyond, no token has a weight
     bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
     auto weight = [&](float l, int i) { return entry_of(l, i) >= first ? row.weight(l) : (u64)0; };
+    const bool plain = first == 0 && row.floor_ > -INFINITY && bucket.per < 1e30f;
     if (first == 0)
-      find_bucket<true>(cl, s, row, bucket, [&](float l, int) { return row.weight(l); }, need_of);
+      find_bucket<true>(cl, s, row, bucket, plain, [&](float l, int) { return row.weight(l); }, need_of);
     else
-      find_bucket<true>(cl, s, row, bucket, weight, need_of);
+      find_bucket<true>(cl, s, row, bucket, false, weight, need_of);
     const float last = (float)s.bucket;
     const u64 want = need_of(s.total), above = s.above;
     // before the border's bucket all stay; the bucket's own go on the list
     if (tid == 0) s.n = 0;
     __syncthreads();
-    const u64 sure = sum_kept(s, row, w0, w1, least, [&](float l, int j) {
+    const float next = last + 1.f;
+    const u64 sure = plain ? sum_kept(s, row, w0, w1, least, [&](float l, int j) {
+      const float at = (bucket.lmax - l) * bucket.per;
+      append(s, l > row.floor_ && at >= last && at < next, l, row.lo + j);
+      return at < last && l >= low;
+    }) : sum_kept(s, row, w0, w1, least, [&](float l, int j) {
       const float at = bucket.place(l);
       const bool in = j < w1 && (first == 0 || entry_of(l, row.lo + j) >= first);
-      append(s, in && at >= last && at < last + 1.f, l, row.lo + j);
+      append(s, in && at >= last && at < next, l, row.lo + j);
       return in && at < last && l >= low;
     });
     if (lane == 0) s.part_lo[warp] = (uint32_t)sure, s.part_hi[warp] = (uint32_t)(sure >> 32);
     const int n = collect(cl, s);
     if (n <= SP_LIST) {
       if (rank == 0) {
-        int N;
-        sort_list(s.ent, n, &N);
+        sort_list(s.ent, n);
         for (int i = tid; i < n; i += SP_THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
         __syncthreads();
         scan_list(s, n, [&](int i) { return s.list.wt[i]; });
