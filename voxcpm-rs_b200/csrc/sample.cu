@@ -43,6 +43,12 @@ constexpr int SP_BITS = 44;          // binary places of a weight
 constexpr double SP_ONE = (double)(1ull << SP_BITS);
 static_assert(SP_MAX_VOCAB == 1 << 18, "the vocabulary that the header names; sums stay below 2^62");
 
+// 2^(i / 16)
+__constant__ double kExpTable[16] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916, 1.189207115002721,
+    1.241857812073484, 1.2968395546510096, 1.3542555469368927, 1.4142135623730951, 1.4768261459394993,
+    1.5422108254079407, 1.6104903319492543, 1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+
 struct SampleArgs {
   const float* logits;
   long long ld;
@@ -210,10 +216,12 @@ __device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& r
   cl.sync();
   if (warp == 0) {
     u64 v[2] = {0, 0};
-    for (int r = 0; r < C; ++r) {
-      const u64* p = cl.map_shared_rank(s.coarse, r) + lane * 2;
-      v[0] += p[0], v[1] += p[1];
-    }
+#pragma unroll
+    for (int r = 0; r < SP_MAX_CLUSTER; ++r)  // unrolled: one round trip for all blocks
+      if (r < C) {
+        const u64* p = cl.map_shared_rank(s.coarse, r) + lane * 2;
+        v[0] += p[0], v[1] += p[1];
+      }
     const u64 incl = warp_scan64(v[0] + v[1]), total = __shfl_sync(0xffffffffu, incl, 31), want = need(total);
     const uint32_t hit = __ballot_sync(0xffffffffu, incl >= want);
     const int at = hit ? __ffs(hit) - 1 : 31;  // (always one: want is at most the total)
@@ -224,8 +232,9 @@ __device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& r
     c = __shfl_sync(0xffffffffu, c, at);
     u64 f = 0;
     const int i = c * (SP_BUCKETS / SP_COARSE) + lane;
-    for (int r = 0; r < C; ++r)
-      f += (u64)cl.map_shared_rank(s.hist.hi, r)[i] << 32 | cl.map_shared_rank(s.hist.lo, r)[i];
+#pragma unroll
+    for (int r = 0; r < SP_MAX_CLUSTER; ++r)
+      if (r < C) f += (u64)cl.map_shared_rank(s.hist.hi, r)[i] << 32 | cl.map_shared_rank(s.hist.lo, r)[i];
     const u64 fi = warp_scan64(f) + above;
     const uint32_t fh = __ballot_sync(0xffffffffu, fi >= want);
     const int b = fh ? __ffs(fh) - 1 : 31;
@@ -255,14 +264,21 @@ __device__ __forceinline__ void append(SampleShared& s, bool in, float l, int in
 __device__ int collect(cg::cluster_group& cl, SampleShared& s) {
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   cl.sync();
-  int n = 0;
-  for (int r = 0; r < C; ++r) {
-    const int c = *cl.map_shared_rank(&s.n, r);
-    if (rank == 0 && r > 0 && n + c <= SP_LIST) {
-      const u64* p = cl.map_shared_rank(s.ent, r);
-      for (int i = threadIdx.x; i < c; i += SP_THREADS) s.ent[n + i] = p[i];
+  int first[SP_MAX_CLUSTER + 1];
+  first[0] = 0;
+#pragma unroll
+  for (int r = 0; r < SP_MAX_CLUSTER; ++r) first[r + 1] = r < C ? *cl.map_shared_rank(&s.n, r) : 0;
+#pragma unroll
+  for (int r = 0; r < SP_MAX_CLUSTER; ++r) first[r + 1] += first[r];
+  const int n = first[SP_MAX_CLUSTER];
+  if (rank == 0 && n <= SP_LIST) {
+    for (int i = first[1] + threadIdx.x; i < n; i += SP_THREADS) {
+      int owner = 0, at = i;
+#pragma unroll
+      for (int r = 1; r < SP_MAX_CLUSTER; ++r)
+        if (i >= first[r]) owner = r, at = i - first[r];
+      s.ent[i] = cl.map_shared_rank(s.ent, owner)[at];
     }
-    n += c;
   }
   __syncthreads();
   return n;
@@ -272,10 +288,18 @@ template <class Take>
 __device__ int gather(cg::cluster_group& cl, SampleShared& s, const Row& row, Take take) {
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
-  for (int j0 = 0; j0 < row.cnt; j0 += SP_THREADS) {
-    const int j = j0 + threadIdx.x;
-    const float l = j < row.cnt ? row.x[j] : -INFINITY;
-    append(s, j < row.cnt && take(l, row.lo + j), l, row.lo + j);
+  constexpr int U = 4;
+  for (int j0 = 0; j0 < row.cnt; j0 += U * SP_THREADS) {
+    float l[U];
+    bool in[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = j0 + i * SP_THREADS + threadIdx.x;
+      l[i] = j < row.cnt ? row.x[j] : -INFINITY;
+      in[i] = j < row.cnt && take(l[i], row.lo + j);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) append(s, in[i], l[i], row.lo + j0 + i * SP_THREADS + threadIdx.x);
   }
   return collect(cl, s);
 }
@@ -311,10 +335,24 @@ __device__ u64 sum_kept(SampleShared& s, const Row& row, int j0, int j1, u64 lea
   return warp_sum64(sum);
 }
 
-// ent[0, n) in descending order (bitonic); entries differ from one another.  A thread has one pair
+// ent[0, n) in descending order; entries differ from one another.  Long lists: bitonic; a thread has one pair
 // of each step; pairs up to 32 apart stay within the 64 entries of a warp, which then needs no
 // barrier with the others.
 __device__ void sort_list(u64* ent, int n) {
+  if (n <= SP_THREADS / 4) {  // short: an entry's place is the number of larger ones, counted by four threads
+    __syncthreads();  // the entries are there
+    const int i = threadIdx.x >> 2;
+    const u64 e = i < n ? ent[i] : 0;
+    int larger = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x & 3; j < n; j += 4) larger += ent[j] > e;
+    larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+    larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+    __syncthreads();
+    if (i < n && (threadIdx.x & 3) == 0) ent[larger] = e;
+    __syncthreads();
+    return;
+  }
   int N = 32;
   while (N < n) N <<= 1;
   for (int i = n + threadIdx.x; i < N; i += SP_THREADS) ent[i] = 0;
@@ -344,9 +382,12 @@ __device__ void scan_list(SampleShared& s, int n, Value value) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const u64 a = 2 * tid < n ? value(2 * tid) : 0, b = 2 * tid + 1 < n ? value(2 * tid + 1) : 0;
   u64 incl = warp_scan64(a + b);
-  if (lane == 31) s.warp64[warp] = incl;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) incl += s.warp64[w];
+  if (n > 64) {  // else all of them are warp 0's
+    if (lane == 31) s.warp64[warp] = incl;
+    __syncthreads();
+    const u64 v = lane < SP_WARPS ? s.warp64[lane] : 0, sum = warp_scan64(v);
+    incl += __shfl_sync(0xffffffffu, sum - v, warp);
+  }
   if (2 * tid < n) s.list.pre[2 * tid] = incl - b;
   if (2 * tid + 1 < n) s.list.pre[2 * tid + 1] = incl;
   __syncthreads();
@@ -437,7 +478,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     if (l > -INFINITY) lo = fminf(lo, l);
     bad |= l != l;
   }
-  if (tid < 16) s.tab[tid] = exp2((double)tid / 16);
+  if (tid < 16) s.tab[tid] = kExpTable[tid];
   hi = warp_max(hi);
   lo = -warp_max(-lo);
   if (lane == 0) s.warp64[warp] = (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo);
@@ -494,7 +535,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
                 [&](u64 total) { return total < (u64)k ? total : (u64)k; });
     const int last = s.bucket;
     const u64 want = s.total < (u64)k ? s.total : (u64)k;  // tokens of -infinity never stay
-    const int n = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket(l) <= last; });
+    const int n = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket.place(l) < (float)(last + 1); });
     if (n <= SP_LIST) {  // all on the sorted list, by one block
       if (rank == 0) {
         sort_list(s.ent, n);
@@ -523,7 +564,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
       return;
     }
     cl.sync();  // the counts are read by all
-    const int in_last = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket(l) == last; });
+    const int in_last = gather(cl, s, row, [&](float l, int) {
+      return l > -INFINITY && bucket.place(l) >= (float)last && bucket.place(l) < (float)(last + 1);
+    });
     if (in_last <= SP_LIST) {
       if (rank == 0) {
         sort_list(s.ent, in_last);
