@@ -154,8 +154,7 @@ int vx_ctx_create(int device, vx_ctx** out) {
       cudaMalloc(&ctx->dev_err, 64) != cudaSuccess || cudaMemset(ctx->dev_err, 0, 64) != cudaSuccess ||
       gemv_configure() != cudaSuccess || tc_gemm_configure() != cudaSuccess ||
       vae_tc_configure() != cudaSuccess || kv4_attend_configure() != cudaSuccess ||
-      kv4_evict_configure() != cudaSuccess ||
-      sample_configure() != cudaSuccess) {
+      kv4_evict_configure() != cudaSuccess || sample_configure() != cudaSuccess) {
     cudaGetLastError();
     delete ctx;
     return VX_ERR_CUDA;

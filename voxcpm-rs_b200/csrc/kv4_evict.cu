@@ -109,16 +109,15 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
     if (tid < 256) s.hist[(p + 1) % 3][tid] = 0;  // last read two passes ago
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const bool mine = base + 32 * i < n && (shift == 24 || ((key[i] ^ T) >> (shift + 8)) == 0);
-      // lanes of the same digit add once: weights share their leading digits
-      const uint32_t d = mine ? (key[i] >> shift) & 255 : 256;
-      const uint32_t same = __match_any_sync(0xffffffffu, d);
-      if (mine && lane == __ffs(same) - 1) atomicAdd(&h[d], (uint32_t)__popc(same));
+      if (base + 32 * i < n && (shift == 24 || ((key[i] ^ T) >> (shift + 8)) == 0))
+        atomicAdd(&h[(key[i] >> shift) & 255], 1u);
     }
     cl.sync();
     if (tid < 256) {
       uint32_t t = 0;
-      for (int r = 0; r < C; ++r) t += cl.map_shared_rank(h, r)[tid];
+#pragma unroll
+      for (int r = 0; r < EV_MAX_CLUSTER; ++r)  // unrolled: one round trip for all blocks
+        if (r < C) t += cl.map_shared_rank(h, r)[tid];
       s.tot[tid] = t;
     }
     __syncthreads();
@@ -201,9 +200,24 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
     if (mover) list[kLast - (mb + __popc(mm & below))] = j;
     hb += __popc(hm);
     mb += __popc(mm);
-    if (keep && j < a.keep) {
-      if (a.weights_out != a.weights) a.weights_out[row0 + j] = a.weights[row0 + j];
-      if (a.positions_out != a.positions) a.positions_out[row0 + j] = a.positions[row0 + j];
+  }
+  // rows that stay where they are: loads of eight at a time, ahead of the stores that may alias them
+  if ((rank * EV_WARPS + warp) * 32 * ITEMS < a.keep && (a.weights_out != a.weights || a.positions_out != a.positions)) {
+    constexpr int G = ITEMS < 8 ? ITEMS : 8;
+#pragma unroll
+    for (int i0 = 0; i0 < ITEMS; i0 += G) {
+      float w[G];
+      int64_t pos[G];
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int j = base + 32 * (i0 + i);
+        if ((stays >> (i0 + i) & 1) && j < a.keep) w[i] = a.weights[row0 + j], pos[i] = a.positions[row0 + j];
+      }
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const int j = base + 32 * (i0 + i);
+        if ((stays >> (i0 + i) & 1) && j < a.keep) a.weights_out[row0 + j] = w[i], a.positions_out[row0 + j] = pos[i];
+      }
     }
   }
   cl.sync();

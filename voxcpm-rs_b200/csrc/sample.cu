@@ -1,6 +1,5 @@
 // Token sampling from logits (vx_sample): temperature, top-k, top-p, min-p and a draw from a
-// given random number, one cluster of C thread blocks per row of logits, the row in their shared
-// memory.
+// given random number, one cluster of thread blocks per row of logits.
 //
 // A token's weight is w = rint(exp((l - lmax) / T) * 2^44) as a 64-bit integer: sums of weights
 // are exact whatever their order (a row of 2^18 tokens stays below 2^62), so every block and
@@ -8,17 +7,18 @@
 // (logit descending, index ascending), described by the last of them, an "entry": the logit's
 // ordered bits above the inverted index.
 //
-// The border is found by counts (top-k) or weights (top-p): a histogram of lmax - l in 2048 equal
+// The border is found by counts (top-k) or weights (top-p): a histogram of lmax - l in equal
 // buckets says in which bucket it lies, and the few entries of that bucket are gathered, sorted
 // and summed by one block.  Where top-k leaves few tokens these are gathered at once, and top-p,
 // min-p and the draw work on the sorted list.  A bucket too full for the list (equal logits, or a
 // border behind the range of the buckets) goes through radix passes over the entries instead.
 // The draw takes the first token in index order whose running sum of staying weights exceeds
-// u * total: sums of each warp's part of the row, then one warp walks its part again.
+// u * total: sums of each warp's part of the row, then one block walks the part that holds it.
 //
-// What bounds it: f64 arithmetic and shared-memory atomics where every token needs its weight
-// (5.8 clocks of an SM for 32 exponentials, 3.7 for their two 32-bit atomics; one 64-bit atomic is
-// a compare-and-swap loop of 30), else the latency of four cluster barriers.
+// What bounds it: where every token needs its weight, instruction issue in two passes (about 45 and
+// 40 instructions of a warp for 32 tokens: 13 f64 operations, a table read, two 32-bit shared-memory
+// atomics, 3.7 clocks of an SM where one 64-bit atomic is a compare-and-swap loop of 30) and, for
+// few rows, the round trips between the blocks (each about half a microsecond; six of them).
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -33,15 +33,11 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32;
 constexpr int SP_MAX_CLUSTER = 8;
-constexpr int SP_SLICE = 32768;      // logits of a block at most: 128 KB
-constexpr int SP_MAX_VOCAB = SP_SLICE * SP_MAX_CLUSTER;
-constexpr int SP_BUCKETS = 2048, SP_COARSE = 64;
-constexpr int SP_LIST = 1024;        // entries that are sorted
+constexpr int SP_MAX_VOCAB = 1 << 18;  // sums of weights stay below 2^62
+constexpr int SP_THREADS = 512;
 constexpr int SP_BITS = 44;          // binary places of a weight
 constexpr double SP_ONE = (double)(1ull << SP_BITS);
-static_assert(SP_MAX_VOCAB == 1 << 18, "the vocabulary that the header names; sums stay below 2^62");
 
 // 2^(i / 16)
 __constant__ double kExpTable[16] = {
@@ -71,34 +67,45 @@ __device__ __forceinline__ float logit_of(u64 entry) {
 }
 __device__ __forceinline__ int index_of(u64 entry) { return 0xffffff - (int)(entry & 0xffffffu); }
 
+// Two forms.  Few rows: the row in shared memory, where three passes read it.  Many rows: read from
+// L2 after the first pass, which leaves room for twice the buckets and so for a shorter list.
+template <bool IN_SHARED>
 struct SampleShared {
+  static constexpr int kThreads = SP_THREADS, kWarps = SP_THREADS / 32;
+  static constexpr int kBuckets = IN_SHARED ? 2048 : 4096, kCoarse = kBuckets / 32;
+  static constexpr int kList = IN_SHARED ? 1024 : 512;  // entries that are sorted
   union {
     struct {
-      uint32_t lo[SP_BUCKETS], hi[SP_BUCKETS];
+      uint32_t lo[kBuckets], hi[kBuckets];
     } hist;
     struct {
-      u64 wt[SP_LIST], pre[SP_LIST];  // of the sorted list: weights, running sums
+      u64 wt[kList], pre[kList];  // of the sorted list: weights, running sums
     } list;
   };
-  u64 ent[SP_LIST];  // gathered entries
+  u64 ent[kList];  // gathered entries
   double tab[16];    // 2^(i / 16)
-  float kept[SP_WARPS][64];               // logits whose weights a warp has yet to sum
-  uint32_t part_lo[SP_WARPS], part_hi[SP_WARPS];  // the sum of each warp's part of the row
-  u64 coarse[SP_COARSE];
-  u64 warp64[SP_WARPS];
+  float kept[kWarps][64];               // logits whose weights a warp has yet to sum
+  uint32_t part_lo[kWarps], part_hi[kWarps];  // the sum of each warp's part of the row
+  u64 coarse[kCoarse];
+  u64 warp64[kWarps];
   u64 total, above, border;
-  uint32_t warp32[SP_WARPS];
+  uint32_t warp32[kWarps];
   float fmax, fmin;
   int bad, bucket, n;
 };
 
 // Everything that the passes over a row share.
+extern __shared__ __align__(16) float shared_row[];
+
+template <bool IN_SHARED>
 struct Row {
   const float* x;  // this block's logits
   int lo, cnt;     // their first index and number
   float lmax, floor_;
   double lmax_d, inv_t;
   const double* tab;
+
+  __device__ __forceinline__ float at(int j) const { return IN_SHARED ? shared_row[j] : __ldg(x + j); }
 
   // exp by a table of 2^(i/16) and a polynomial of degree 6 (table-driven, after Tang, 1989): off by
   // less than 2^-50 of itself.  16 table entries of 8 bytes are all banks of shared memory once: a
@@ -153,10 +160,11 @@ __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, u64 v) {
 }
 
 // Equal buckets of lmax - l: at `per` buckets to a unit, the last one holds the rest.
+template <class Shared>
 struct Buckets {
   float lmax, per;
   __device__ __forceinline__ float place(float l) const {
-    return l == lmax ? 0.f : fminf((lmax - l) * per, (float)(SP_BUCKETS - 1));
+    return l == lmax ? 0.f : fminf((lmax - l) * per, (float)(Shared::kBuckets - 1));
   }
   __device__ __forceinline__ int operator()(float l) const { return (int)place(l); }
 };
@@ -164,20 +172,20 @@ struct Buckets {
 // The histogram over the cluster of value(l, index) and the bucket in which the running sum from
 // the largest logit on reaches need(total): s.bucket, s.above (the sum before it), s.total.  Every
 // block finds the same.
-template <bool wide, class Value, class Need>
-__device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& row, const Buckets& bucket, bool plain,
+template <bool wide, class Shared, class R, class Value, class Need>
+__device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, const Buckets<Shared>& bucket, bool plain,
                             Value value, Need need) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = (int)cl.num_blocks();
-  for (int i = tid; i < SP_BUCKETS; i += SP_THREADS) s.hist.lo[i] = s.hist.hi[i] = 0;
+  for (int i = tid; i < Shared::kBuckets; i += Shared::kThreads) s.hist.lo[i] = s.hist.hi[i] = 0;
   __syncthreads();
   constexpr int U = 4;  // logits of a thread whose weights are computed together
   int j0 = tid;
   if (plain) {  // `per` is finite and no logit above the floor lies behind the last bucket
-    for (; j0 - tid + U * SP_THREADS <= row.cnt; j0 += U * SP_THREADS) {
+    for (; j0 - tid + U * Shared::kThreads <= row.cnt; j0 += U * Shared::kThreads) {
       float l[U];
       u64 v[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) l[i] = row.x[j0 + i * SP_THREADS];
+      for (int i = 0; i < U; ++i) l[i] = row.at(j0 + i * Shared::kThreads);
 #pragma unroll
       for (int i = 0; i < U; ++i) v[i] = row.exp_of(((double)fmaxf(l[i], row.floor_) - row.lmax_d) * row.inv_t);
 #pragma unroll
@@ -188,13 +196,13 @@ __device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& r
         }
     }
   }
-  for (; j0 < row.cnt; j0 += U * SP_THREADS) {
+  for (; j0 < row.cnt; j0 += U * Shared::kThreads) {
     u64 v[U];
     int at[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int j = j0 + i * SP_THREADS;
-      const float l = j < row.cnt ? row.x[j] : -INFINITY;
+      const int j = j0 + i * Shared::kThreads;
+      const float l = j < row.cnt ? row.at(j) : -INFINITY;
       v[i] = l > -INFINITY ? value(l, row.lo + j) : 0;
       at[i] = bucket(l);
     }
@@ -208,30 +216,39 @@ __device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& r
       }
   }
   __syncthreads();
-  for (int c = warp; c < SP_COARSE; c += SP_WARPS) {
-    const int i = c * (SP_BUCKETS / SP_COARSE) + lane;
+  for (int c = warp; c < Shared::kCoarse; c += Shared::kWarps) {
+    const int i = c * (Shared::kBuckets / Shared::kCoarse) + lane;
     const u64 v = warp_sum64((u64)s.hist.hi[i] << 32 | s.hist.lo[i]);
     if (lane == 0) s.coarse[c] = v;
   }
   cl.sync();
   if (warp == 0) {
-    u64 v[2] = {0, 0};
+    constexpr int CL = Shared::kCoarse / 32;  // coarse sums of a lane
+    u64 v[CL] = {}, sum = 0;
 #pragma unroll
     for (int r = 0; r < SP_MAX_CLUSTER; ++r)  // unrolled: one round trip for all blocks
       if (r < C) {
-        const u64* p = cl.map_shared_rank(s.coarse, r) + lane * 2;
-        v[0] += p[0], v[1] += p[1];
+        const u64* p = cl.map_shared_rank(s.coarse, r) + lane * CL;
+#pragma unroll
+        for (int e = 0; e < CL; ++e) v[e] += p[e];
       }
-    const u64 incl = warp_scan64(v[0] + v[1]), total = __shfl_sync(0xffffffffu, incl, 31), want = need(total);
+#pragma unroll
+    for (int e = 0; e < CL; ++e) sum += v[e];
+    const u64 incl = warp_scan64(sum), total = __shfl_sync(0xffffffffu, incl, 31), want = need(total);
     const uint32_t hit = __ballot_sync(0xffffffffu, incl >= want);
     const int at = hit ? __ffs(hit) - 1 : 31;  // (always one: want is at most the total)
-    u64 above = incl - v[0] - v[1];
-    int c = lane * 2;
-    if (above + v[0] < want) above += v[0], ++c;
+    u64 above = incl - sum;
+    int c = lane * CL;
+    bool past = true;
+#pragma unroll
+    for (int e = 0; e < CL - 1; ++e) {
+      past = past && above + v[e] < want;
+      if (past) above += v[e], ++c;
+    }
     above = __shfl_sync(0xffffffffu, above, at);
     c = __shfl_sync(0xffffffffu, c, at);
     u64 f = 0;
-    const int i = c * (SP_BUCKETS / SP_COARSE) + lane;
+    const int i = c * (Shared::kBuckets / Shared::kCoarse) + lane;
 #pragma unroll
     for (int r = 0; r < SP_MAX_CLUSTER; ++r)
       if (r < C) f += (u64)cl.map_shared_rank(s.hist.hi, r)[i] << 32 | cl.map_shared_rank(s.hist.lo, r)[i];
@@ -240,7 +257,7 @@ __device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& r
     const int b = fh ? __ffs(fh) - 1 : 31;
     const u64 before = __shfl_sync(0xffffffffu, fi - f, b);
     if (lane == 0) {
-      s.bucket = c * (SP_BUCKETS / SP_COARSE) + b;
+      s.bucket = c * (Shared::kBuckets / Shared::kCoarse) + b;
       s.above = before;
       s.total = total;
     }
@@ -249,19 +266,21 @@ __device__ void find_bucket(cg::cluster_group& cl, SampleShared& s, const Row& r
 }
 
 // A warp's lanes for which `in` holds put their entries behind this block's others.
-__device__ __forceinline__ void append(SampleShared& s, bool in, float l, int index) {
+template <class Shared>
+__device__ __forceinline__ void append(Shared& s, bool in, float l, int index) {
   const uint32_t m = __ballot_sync(0xffffffffu, in);
   if (m == 0) return;
   const int lane = threadIdx.x & 31;
   int at = 0;
   if (lane == __ffs(m) - 1) at = atomicAdd(&s.n, __popc(m));
   at = __shfl_sync(0xffffffffu, at, __ffs(m) - 1) + __popc(m & ((1u << lane) - 1));
-  if (in && at < SP_LIST) s.ent[at] = entry_of(l, index);
+  if (in && at < Shared::kList) s.ent[at] = entry_of(l, index);
 }
 
 // The blocks' entries, in no order, in block 0's s.ent; their number, the same for all.  Above
-// SP_LIST the list is of no use.
-__device__ int collect(cg::cluster_group& cl, SampleShared& s) {
+// Shared::kList the list is of no use.
+template <class Shared>
+__device__ int collect(cg::cluster_group& cl, Shared& s) {
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   cl.sync();
   int first[SP_MAX_CLUSTER + 1];
@@ -271,8 +290,8 @@ __device__ int collect(cg::cluster_group& cl, SampleShared& s) {
 #pragma unroll
   for (int r = 0; r < SP_MAX_CLUSTER; ++r) first[r + 1] += first[r];
   const int n = first[SP_MAX_CLUSTER];
-  if (rank == 0 && n <= SP_LIST) {
-    for (int i = first[1] + threadIdx.x; i < n; i += SP_THREADS) {
+  if (rank == 0 && n <= Shared::kList) {
+    for (int i = first[1] + threadIdx.x; i < n; i += Shared::kThreads) {
       int owner = 0, at = i;
 #pragma unroll
       for (int r = 1; r < SP_MAX_CLUSTER; ++r)
@@ -284,30 +303,30 @@ __device__ int collect(cg::cluster_group& cl, SampleShared& s) {
   return n;
 }
 
-template <class Take>
-__device__ int gather(cg::cluster_group& cl, SampleShared& s, const Row& row, Take take) {
+template <class Shared, class R, class Take>
+__device__ int gather(cg::cluster_group& cl, Shared& s, const R& row, Take take) {
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   constexpr int U = 4;
-  for (int j0 = 0; j0 < row.cnt; j0 += U * SP_THREADS) {
+  for (int j0 = 0; j0 < row.cnt; j0 += U * Shared::kThreads) {
     float l[U];
     bool in[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int j = j0 + i * SP_THREADS + threadIdx.x;
-      l[i] = j < row.cnt ? row.x[j] : -INFINITY;
+      const int j = j0 + i * Shared::kThreads + threadIdx.x;
+      l[i] = j < row.cnt ? row.at(j) : -INFINITY;
       in[i] = j < row.cnt && take(l[i], row.lo + j);
     }
 #pragma unroll
-    for (int i = 0; i < U; ++i) append(s, in[i], l[i], row.lo + j0 + i * SP_THREADS + threadIdx.x);
+    for (int i = 0; i < U; ++i) append(s, in[i], l[i], row.lo + j0 + i * Shared::kThreads + threadIdx.x);
   }
   return collect(cl, s);
 }
 
 // The sum of the weights, where at least `least`, of the logits j in [j0, j1) for which keep(l, j)
 // holds, by one warp.  The few that are kept are first put side by side, 32 for each exponential.
-template <class Keep>
-__device__ u64 sum_kept(SampleShared& s, const Row& row, int j0, int j1, u64 least, Keep keep) {
+template <class Shared, class R, class Keep>
+__device__ u64 sum_kept(Shared& s, const R& row, int j0, int j1, u64 least, Keep keep) {
   const int lane = threadIdx.x & 31;
   float* buf = s.kept[threadIdx.x >> 5];
   int n = 0;
@@ -317,7 +336,7 @@ __device__ u64 sum_kept(SampleShared& s, const Row& row, int j0, int j1, u64 lea
     if (w >= least) sum += w;
   };
   for (int j = j0 + lane; j - lane < j1; j += 32) {
-    const float l = j < j1 ? row.x[j] : -INFINITY;
+    const float l = j < j1 ? row.at(j) : -INFINITY;
     const bool in = keep(l, j) && j < j1;
     const uint32_t m = __ballot_sync(0xffffffffu, in);
     if (in) buf[n + __popc(m & ((1u << lane) - 1))] = l;
@@ -338,8 +357,10 @@ __device__ u64 sum_kept(SampleShared& s, const Row& row, int j0, int j1, u64 lea
 // ent[0, n) in descending order; entries differ from one another.  Long lists: bitonic; a thread has one pair
 // of each step; pairs up to 32 apart stay within the 64 entries of a warp, which then needs no
 // barrier with the others.
-__device__ void sort_list(u64* ent, int n) {
-  if (n <= SP_THREADS / 4) {  // short: an entry's place is the number of larger ones, counted by four threads
+template <class Shared>
+__device__ void sort_list(Shared& s, int n) {
+  u64* ent = s.ent;
+  if (n <= Shared::kThreads / 4) {  // short: an entry's place is the number of larger ones, counted by four threads
     __syncthreads();  // the entries are there
     const int i = threadIdx.x >> 2;
     const u64 e = i < n ? ent[i] : 0;
@@ -355,9 +376,9 @@ __device__ void sort_list(u64* ent, int n) {
   }
   int N = 32;
   while (N < n) N <<= 1;
-  for (int i = n + threadIdx.x; i < N; i += SP_THREADS) ent[i] = 0;
+  for (int i = n + threadIdx.x; i < N; i += Shared::kThreads) ent[i] = 0;
   __syncthreads();
-  static_assert(SP_LIST / 2 <= SP_THREADS, "a pair for each thread");
+  static_assert(Shared::kList / 2 <= Shared::kThreads, "a pair for each thread");
   const int i = threadIdx.x;
   if (i < (N / 2 + 31) / 32 * 32 || N > 64) {  // whole warps; all of them where they meet at barriers
     for (int k = 2; k <= N; k <<= 1)
@@ -376,16 +397,16 @@ __device__ void sort_list(u64* ent, int n) {
   __syncthreads();
 }
 
-// pre[i] = value(0) + .. + value(i) for i < n <= 2 * SP_THREADS.
-template <class Value>
-__device__ void scan_list(SampleShared& s, int n, Value value) {
+// pre[i] = value(0) + .. + value(i) for i < n <= 2 * Shared::kThreads.
+template <class Shared, class Value>
+__device__ void scan_list(Shared& s, int n, Value value) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const u64 a = 2 * tid < n ? value(2 * tid) : 0, b = 2 * tid + 1 < n ? value(2 * tid + 1) : 0;
   u64 incl = warp_scan64(a + b);
   if (n > 64) {  // else all of them are warp 0's
     if (lane == 31) s.warp64[warp] = incl;
     __syncthreads();
-    const u64 v = lane < SP_WARPS ? s.warp64[lane] : 0, sum = warp_scan64(v);
+    const u64 v = lane < Shared::kWarps ? s.warp64[lane] : 0, sum = warp_scan64(v);
     incl += __shfl_sync(0xffffffffu, sum - v, warp);
   }
   if (2 * tid < n) s.list.pre[2 * tid] = incl - b;
@@ -394,7 +415,8 @@ __device__ void scan_list(SampleShared& s, int n, Value value) {
 }
 
 // The number of leading list entries whose running sum s.list.pre is below `want`.
-__device__ int count_below(SampleShared& s, int n, u64 want) {
+template <class Shared>
+__device__ int count_below(Shared& s, int n, u64 want) {
   const int tid = threadIdx.x;
   return __syncthreads_count(2 * tid < n && s.list.pre[2 * tid] < want) +
          __syncthreads_count(2 * tid + 1 < n && s.list.pre[2 * tid + 1] < want);
@@ -402,8 +424,8 @@ __device__ int count_below(SampleShared& s, int n, u64 want) {
 
 // The smallest entry X for which the sum of value(l, index) over the entries >= X reaches `need`, by
 // radix passes over the 56 bits of an entry; for any number of entries and equal logits.
-template <class Value>
-__device__ u64 radix_border(cg::cluster_group& cl, SampleShared& s, const Row& row, u64 need, Value value) {
+template <class Shared, class R, class Value>
+__device__ u64 radix_border(cg::cluster_group& cl, Shared& s, const R& row, u64 need, Value value) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = (int)cl.num_blocks();
   u64 prefix = 0;
   for (int shift = 48, p = 0; shift >= 0; shift -= 8, ++p) {
@@ -411,8 +433,8 @@ __device__ u64 radix_border(cg::cluster_group& cl, SampleShared& s, const Row& r
     cl.sync();  // the pass before last is read by all
     if (tid < 256) lo[tid] = hi[tid] = 0;
     __syncthreads();
-    for (int j = tid; j < row.cnt; j += SP_THREADS) {
-      const float l = row.x[j];
+    for (int j = tid; j < row.cnt; j += Shared::kThreads) {
+      const float l = row.at(j);
       const u64 e = entry_of(l, row.lo + j);
       if (((e ^ prefix) >> 8) >> shift) continue;
       const u64 v = value(l, row.lo + j);
@@ -451,18 +473,19 @@ __device__ u64 radix_border(cg::cluster_group& cl, SampleShared& s, const Row& r
   return prefix;
 }
 
+template <bool IN_SHARED>
 __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs a) {
-  extern __shared__ __align__(16) float x[];
-  __shared__ SampleShared s;
+  typedef SampleShared<IN_SHARED> Shared;
+  constexpr int THREADS = SP_THREADS, kWarps = Shared::kWarps;
+  __shared__ Shared s;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   const int r = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  Row row;
-  row.x = x;
+  Row<IN_SHARED> row;
   row.lo = min(a.vocab, rank * a.slice);
   row.cnt = min(a.vocab, row.lo + a.slice) - row.lo;
   row.tab = s.tab;
-  const float* src = a.logits + (size_t)r * a.ld + row.lo;
+  row.x = a.logits + (size_t)r * a.ld + row.lo;
   const float temp = a.temperature ? a.temperature[r] : 1.f, p = a.top_p ? a.top_p[r] : 1.f;
   const float mp = a.min_p ? a.min_p[r] : 0.f, uf = a.u[r];
   int k = a.top_k ? a.top_k[r] : 0;
@@ -471,9 +494,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   float hi = -INFINITY, lo = INFINITY;
   bool bad = false;
 #pragma unroll 8
-  for (int j = tid; j < row.cnt; j += SP_THREADS) {
-    const float l = __ldcs(src + j);
-    x[j] = l;
+  for (int j = tid; j < row.cnt; j += THREADS) {
+    const float l = __ldg(row.x + j);
+    if (IN_SHARED) shared_row[j] = l;
     hi = fmaxf(hi, l);
     if (l > -INFINITY) lo = fminf(lo, l);
     bad |= l != l;
@@ -484,7 +507,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   if (lane == 0) s.warp64[warp] = (u64)__float_as_uint(hi) << 32 | __float_as_uint(lo);
   bad = __syncthreads_or(bad);
   if (tid < 32) {
-    const u64 v = s.warp64[lane % SP_WARPS];
+    const u64 v = s.warp64[lane % kWarps];
     hi = warp_max(__uint_as_float((uint32_t)(v >> 32)));
     lo = -warp_max(-__uint_as_float((uint32_t)v));
     if (tid == 0) s.fmax = hi, s.fmin = lo, s.bad = bad;
@@ -528,19 +551,19 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
 
   u64 border = 0;  // entries >= border stay
   if (k > 0) {
-    Buckets bucket = {hi, 0.f};
+    Buckets<Shared> bucket = {hi, 0.f};
     const float range = fminf(hi - lo, 64.f * fmaxf(1.f, greedy ? 1.f : temp));
-    bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
+    bucket.per = range > 0.f ? (Shared::kBuckets - 1) / range : 0.f;
     find_bucket<false>(cl, s, row, bucket, false, [](float, int) { return (u64)1; },
                 [&](u64 total) { return total < (u64)k ? total : (u64)k; });
     const int last = s.bucket;
     const u64 want = s.total < (u64)k ? s.total : (u64)k;  // tokens of -infinity never stay
     const int n = gather(cl, s, row, [&](float l, int) { return l > -INFINITY && bucket.place(l) < (float)(last + 1); });
-    if (n <= SP_LIST) {  // all on the sorted list, by one block
+    if (n <= Shared::kList) {  // all on the sorted list, by one block
       if (rank == 0) {
-        sort_list(s.ent, n);
+        sort_list(s, n);
         int m = (int)want;
-        for (int i = tid; i < m; i += SP_THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
+        for (int i = tid; i < m; i += THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
         __syncthreads();
         scan_list(s, m, [&](int i) { return s.list.wt[i]; });
         if (p < 1.f) m = count_below(s, m, need_of(s.list.pre[m - 1])) + 1;
@@ -550,8 +573,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
         const u64 total = s.list.pre[m - 1], at = drawn(total);
         __syncthreads();
         // index order: entries become (index, place), inverted since the sort descends
-        for (int i = tid; i < m; i += SP_THREADS) s.ent[i] = ~((u64)index_of(s.ent[i]) << 32 | (uint32_t)i);
-        sort_list(s.ent, m);
+        for (int i = tid; i < m; i += THREADS) s.ent[i] = ~((u64)index_of(s.ent[i]) << 32 | (uint32_t)i);
+        sort_list(s, m);
         scan_list(s, m, [&](int i) { return s.list.wt[(uint32_t)~s.ent[i]]; });
         const int place = count_below(s, m, at + 1);
         if (tid == 0) {
@@ -567,9 +590,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     const int in_last = gather(cl, s, row, [&](float l, int) {
       return l > -INFINITY && bucket.place(l) >= (float)last && bucket.place(l) < (float)(last + 1);
     });
-    if (in_last <= SP_LIST) {
+    if (in_last <= Shared::kList) {
       if (rank == 0) {
-        sort_list(s.ent, in_last);
+        sort_list(s, in_last);
         if (tid == 0) s.border = s.ent[(int)(want - s.above) - 1];
       }
       cl.sync();
@@ -580,16 +603,16 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     }
   }
   // each warp has a part of this block's logits; what min-p lets go of for certain needs no weight
-  const int part = max(32, (row.cnt + SP_WARPS * 32 - 1) / (SP_WARPS * 32) * 32);
+  const int part = max(32, (row.cnt + kWarps * 32 - 1) / (kWarps * 32) * 32);
   const int w0 = min(row.cnt, warp * part), w1 = min(row.cnt, w0 + part);
   const float cut = least ? (float)(row.lmax_d + (log(fmin((double)mp, 1.0)) - 1e-3) / row.inv_t) : -INFINITY;
   const float low = cut > -INFINITY ? nextafterf(cut, -INFINITY) : -INFINITY;  // (NaN and +infinity: no cut below)
   bool summed = false;
   if (p < 1.f) {
     const u64 first = border;
-    Buckets bucket = {hi, 0.f};
+    Buckets<Shared> bucket = {hi, 0.f};
     const float range = fminf(hi - lo, (float)(32.1 / row.inv_t));  // beyond, no token has a weight
-    bucket.per = range > 0.f ? (SP_BUCKETS - 1) / range : 0.f;
+    bucket.per = range > 0.f ? (Shared::kBuckets - 1) / range : 0.f;
     auto weight = [&](float l, int i) { return entry_of(l, i) >= first ? row.weight(l) : (u64)0; };
     const bool plain = first == 0 && row.floor_ > -INFINITY && bucket.per < 1e30f;
     if (first == 0)
@@ -614,10 +637,10 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     });
     if (lane == 0) s.part_lo[warp] = (uint32_t)sure, s.part_hi[warp] = (uint32_t)(sure >> 32);
     const int n = collect(cl, s);
-    if (n <= SP_LIST) {
+    if (n <= Shared::kList) {
       if (rank == 0) {
-        sort_list(s.ent, n);
-        for (int i = tid; i < n; i += SP_THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
+        sort_list(s, n);
+        for (int i = tid; i < n; i += THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
         __syncthreads();
         scan_list(s, n, [&](int i) { return s.list.wt[i]; });
         const int place = count_below(s, n, want - above);
@@ -627,7 +650,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
       border = *cl.map_shared_rank(&s.border, 0);
       // those of the list that stay and lie in this block join their warp's sum
       const int own = rank == 0 ? n : s.n;
-      for (int i = tid; i < own; i += SP_THREADS) {
+      for (int i = tid; i < own; i += THREADS) {
         const u64 e = s.ent[i];
         const int j = index_of(e) - row.lo;
         if (e < border || j < 0 || j >= row.cnt) continue;
@@ -657,7 +680,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   __syncthreads();
   u64 before = 0;
   {
-    const u64 v = lane < SP_WARPS ? s.warp64[lane] : 0;
+    const u64 v = lane < kWarps ? s.warp64[lane] : 0;
     const u64 incl = warp_scan64(v);
     before = __shfl_sync(0xffffffffu, incl - v, warp);
     if (tid == 31) s.total = incl;
@@ -677,14 +700,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   if (s.n >= 0) {  // one block of the cluster: all its warps walk the part of that warp
     u64 run = s.above;
     const int j0 = s.n * part, j1 = min(row.cnt, j0 + part);
-    for (int j = j0 + tid; j - tid < j1; j += SP_THREADS) {
-      u64 w = j < j1 && stays(x[j], j) ? row.weight(x[j]) : 0;
+    for (int j = j0 + tid; j - tid < j1; j += THREADS) {
+      u64 w = j < j1 && stays(row.at(j), j) ? row.weight(row.at(j)) : 0;
       if (w < least) w = 0;
       u64 incl = warp_scan64(w);
       __syncthreads();  // warp64 of the round before is read
       if (lane == 31) s.warp64[warp] = incl;
       __syncthreads();
-      for (int q = 0; q < SP_WARPS; ++q) {
+      for (int q = 0; q < kWarps; ++q) {
         if (q == warp) incl += run;
         run += s.warp64[q];
       }
@@ -698,17 +721,29 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   cl.sync();  // the other blocks have read this one's sum
 }
 
-// Blocks of a row: slices that leave room for two blocks on an SM, and more where there are few rows.
-int cluster_of(int rows, int vocab) {
-  int c = 1;
-  while (c < SP_MAX_CLUSTER && (vocab > 19456 * c || (rows * c < 148 && vocab > 2048 * c))) c *= 2;
-  return c;
+// Blocks of a row, and whether they hold it in shared memory.
+struct SampleShape {
+  int blocks;
+  bool in_shared;
+};
+constexpr int SP_SLICE = 32768;  // logits of a block in shared memory at most: 128 KB
+constexpr int SP_TWO = 18432;    // that leave room for two blocks on an SM
+// As many blocks of a row as there are SMs for (one row of 73448 tokens: 8 blocks 15 us, 2 blocks
+// 27 us; 64 rows: 4 blocks 38 us, 8 blocks 52 us).  256 rows of 151643 tokens: 2 blocks that read L2
+// 288 us, 8 with the row in shared memory 347 us.
+SampleShape shape_of(int rows, int vocab) {
+  SampleShape p = {1, true};
+  while (p.blocks < SP_MAX_CLUSTER && vocab > 2048 * p.blocks && rows * p.blocks < 148) p.blocks *= 2;
+  const int slice = (vocab + p.blocks - 1) / p.blocks;
+  p.in_shared = slice <= SP_TWO || (slice <= SP_SLICE && rows * p.blocks <= 148);
+  if (!p.in_shared && p.blocks == 1) p.blocks = 2;
+  return p;
 }
 
 }  // namespace
 
 cudaError_t sample_configure() {
-  return cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_SLICE * 4);
+  return cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_SLICE * 4);
 }
 
 }  // namespace vx
@@ -725,22 +760,23 @@ extern "C" int vx_sample(vx_ctx* ctx, const float* logits, int64_t row_stride, i
   if (row_stride < vocab) return fail(ctx, VX_ERR_SHAPE, "sample: row stride below the vocabulary");
   if (rows == 0) return VX_OK;
   DeviceGuard guard(ctx->device);
-  const int C = cluster_of(rows, vocab);
-  SampleArgs a = {logits, row_stride, rows, vocab, (vocab + C - 1) / C, u, temperature, top_k, top_p, min_p, ids,
-                  logprob};
+  const SampleShape p = shape_of(rows, vocab);
+  SampleArgs a = {logits, row_stride, rows, vocab, (vocab + p.blocks - 1) / p.blocks, u, temperature, top_k, top_p,
+                  min_p, ids, logprob};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows * C);
+  cfg.gridDim = dim3(rows * p.blocks);
   cfg.blockDim = dim3(SP_THREADS);
-  cfg.dynamicSmemBytes = (size_t)a.slice * 4;
+  cfg.dynamicSmemBytes = p.in_shared ? (size_t)a.slice * 4 : 0;
   cfg.stream = pick_stream(ctx, stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.x = p.blocks;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  VX_CUDA(ctx, cudaLaunchKernelEx(&cfg, sample_kernel, a));
+  VX_CUDA(ctx, p.in_shared ? cudaLaunchKernelEx(&cfg, sample_kernel<true>, a)
+                           : cudaLaunchKernelEx(&cfg, sample_kernel<false>, a));
   return VX_OK;
 }
