@@ -320,49 +320,49 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 4 : 5) kv4_split_ker
       s[i] = ex2(s[i] - m);
       l += s[i];
     }
+    uint32_t ph[2][2], pl[2][2], sc[2][2];  // 16-position block, n-tile of S in it
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {  // 16 positions
-      uint32_t ph[2], pl[2];
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float x = s[4 * k + 2 * i], y = s[4 * k + 2 * i + 1];
-        ph[i] = pack_h2(x, y);
-        pl[i] = pack_h2(x - h2_lo(ph[i]), y - h2_hi(ph[i]));
-      }
-      constexpr int NW = D / 64;  // words of a thread's piece of a row
-      uint32_t w[4][NW], sc[2];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // n-tile e / 2, column 2t + e % 2
-        const uint8_t* p = st + v_off[e & 1] + (2 * k + (e >> 1)) * 8 * (D / 2);
-        if constexpr (D == 128) {
-          const uint2 v = *reinterpret_cast<const uint2*>(p);
-          w[e][0] = v.x, w[e][NW - 1] = v.y;
-        } else {
-          w[e][0] = *reinterpret_cast<const uint32_t*>(p);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
+        ph[k][i] = pack_h2(x, y);
+        pl[k][i] = pack_h2(x - h2_lo(ph[k][i]), y - h2_hi(ph[k][i]));
         const uint8_t* p = st + (2 * k + i) * 8 * (D / 16);
-        sc[i] = e4m3x2_to_h2((uint32_t)p[vs_off[0]] | (uint32_t)p[vs_off[1]] << 8);
+        sc[k][i] = e4m3x2_to_h2((uint32_t)p[vs_off[0]] | (uint32_t)p[vs_off[1]] << 8);
       }
+    // The tile's products start from zero and join the running sums by plain additions: the tensor
+    // core's own additions drop bits, always towards zero, and hundreds of them in a row were off
+    // by 2e-6 of the result.
 #pragma unroll
-      for (int q = 0; q < NW; ++q) {
+    for (int q = 0; q < D / 64; ++q) {  // words of a thread's piece of a row
+      float c[4][4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
         uint32_t ev[2][4], od[2][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t x = w[2 * i][q], y = w[2 * i + 1][q];
+        for (int i = 0; i < 2; ++i) {  // columns 2t and 2t + 1 of an n-tile
+          const uint8_t* p = st + (2 * k + i) * 8 * (D / 2) + 4 * q;
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(p + v_off[0]);
+          const uint32_t y = *reinterpret_cast<const uint32_t*>(p + v_off[1]);
           e2m1x8_to_h2((x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u), ev[i]);
           e2m1x8_to_h2(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), od[i]);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t a0 = mul_h2(ev[0][j], sc[0]), a1 = mul_h2(od[0][j], sc[0]), a2 = mul_h2(ev[1][j], sc[1]),
-                         a3 = mul_h2(od[1][j], sc[1]);
-          mma_16816(o[4 * q + j], a0, a1, a2, a3, ph[0], ph[1]);
-          mma_16816(o[4 * q + j], a0, a1, a2, a3, pl[0], pl[1]);
+          const uint32_t a0 = mul_h2(ev[0][j], sc[k][0]), a1 = mul_h2(od[0][j], sc[k][0]),
+                         a2 = mul_h2(ev[1][j], sc[k][1]), a3 = mul_h2(od[1][j], sc[k][1]);
+          if (k == 0)
+            mma_16816_zero(c[j], a0, a1, a2, a3, ph[0][0], ph[0][1]);
+          else
+            mma_16816(c[j], a0, a1, a2, a3, ph[1][0], ph[1][1]);
+          mma_16816(c[j], a0, a1, a2, a3, pl[k][0], pl[k][1]);
         }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[4 * q + j][e] += c[j][e];
     }
     __syncwarp();  // every lane has read the stage that the next load goes into
     const int nx = it + AT_STAGES - 1;
