@@ -292,6 +292,15 @@ int vx_lm_layer_forward_step(vx_lm* lm, int layer, float* hidden, int pos);
  * prefill's last row).  The decode step runs as one captured CUDA graph replayed per step
  * with no host round trip; cancellation (vx_cancel) is polled between steps. */
 int vx_lm_greedy(vx_lm* lm, const int32_t* prompt_ids, int n_prompt, int n_steps, int32_t* tokens_out);
+/* vx_lm_greedy's loop for B prompts of equal length (prompt_ids [B][n_prompt], host) with every
+ * pick drawn from the row's logits by vx_sample: u [n_steps + 1][B] in [0, 1) and the rows'
+ * settings [B] (NULL: off) are host or device arrays; temperature 0 picks the largest.
+ * tokens_out (host) receives [B][n_steps + 1] ids (-1 where a row's logits hold a NaN; the
+ * loop goes on from id 0).  Runs the batched step (VX_ERR_SHAPE above max_batch or 128 rows);
+ * vx_cancel is polled between steps. */
+int vx_lm_sample(vx_lm* lm, const int32_t* prompt_ids, int B, int n_prompt, int n_steps, const float* u,
+                 const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                 int32_t* tokens_out);
 /* One batch-1 decode step at `pos` run eagerly (no graph, no programmatic dependent launch)
  * with a CUDA event after every kernel: kernel_us receives num_hidden_layers*5 + 1 durations
  * (per layer: qkv+rope, attention, o_proj, gate_up, down; then the greedy head).  Writes the

@@ -23,6 +23,7 @@ def test_null_arguments_are_refused():
     assert L.vx_kv4_read(None, ref, 1, None, None, None, None, None) == _lib.VX_ERR_ARG
     assert L.vx_kv4_attend(None, ref, None, 0, 1, None, 1, 1.0, 0, None, 0, None, 0, None) == _lib.VX_ERR_ARG
     assert L.vx_kv4_evict(None, ref, None, None, 1, 1, 0, 0, None, None, None, None) == _lib.VX_ERR_ARG
+    assert L.vx_lm_sample(None, None, 1, 1, 1, None, None, None, None, None, None) == _lib.VX_ERR_ARG
     assert L.vx_sample(None, None, 1, 1, 1, None, None, None, None, None, None, None, None) == _lib.VX_ERR_ARG
 
 

@@ -344,6 +344,23 @@ __global__ void advance_kernel(int* pos, int* step, int inc_pos) {
   *step += 1;
 }
 
+// The sampled counterpart of the pick above: the ids are given.
+__global__ void __launch_bounds__(256) take_ids_kernel(const int* __restrict__ ids, int V, const int* step, int* tokens,
+                                                       int ld_tokens, const uint16_t* __restrict__ E, int H,
+                                                       float scale, float* next_x) {
+  const int b = blockIdx.x, id = ids[b];
+  if (threadIdx.x == 0) tokens[(size_t)(*step) * ld_tokens + b] = id;
+  const uint16_t* e = E + (size_t)(id < 0 || id >= V ? 0 : id) * H;
+  for (int k = threadIdx.x; k < H; k += 256) next_x[(size_t)b * H + k] = __uint_as_float(((uint32_t)e[k]) << 16) * scale;
+}
+
+cudaError_t launch_take_ids(const int* ids, int B, int V, const int* step, int* tokens, int ld_tokens,
+                            const uint16_t* E, int H, float scale, float* next_x, cudaStream_t st) {
+  count_launch();
+  take_ids_kernel<<<B, 256, 0, st>>>(ids, V, step, tokens, ld_tokens, E, H, scale, next_x);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_argmax_rows(const float* logits, int B, int V, const int* step, int* tokens, int ld_tokens,
                                const uint16_t* E, int H, float scale, float* next_x, cudaStream_t st) {
   count_launch();

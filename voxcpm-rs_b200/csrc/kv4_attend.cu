@@ -689,8 +689,8 @@ int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* c, const float* q, int64_t q_stride
     return fail(ctx, VX_ERR_SHAPE, "kv4_attend: max_len %d outside 0..%d", max_len, c->capacity);
   if (track && !c->weights) return fail(ctx, VX_ERR_ARG, "kv4_attend: the cache keeps no weights to add to");
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || q_stride % 4 != 0 || out_stride % 4 != 0 ||
-      q_stride < (int64_t)nh * c->head_dim || out_stride < (int64_t)nh * c->head_dim)
-    return fail(ctx, VX_ERR_ARG, "kv4_attend: q and out must be 16-byte aligned rows of nh * head_dim floats");
+      out_stride < (int64_t)nh * c->head_dim)
+    return fail(ctx, VX_ERR_ARG, "kv4_attend: the rows of q and out must be 16-byte aligned, those of out not overlap");
   const AttendPlan p = plan_of(c, nh, max_len, track);
   const size_t need = p.need();
   if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))

@@ -22,6 +22,16 @@ using namespace vx;
 
 namespace {
 
+// Device arrays of a sampling call (vx_lm_sample): the rows' settings (null: off) and the random
+// numbers of every pick, [picks][B].
+struct LmSampling {
+  const float* u;
+  const float* temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p;
+  int32_t* ids;
+};
+
 struct LmLayer {
   uint16_t* wqkv = nullptr;
   uint16_t* wo = nullptr;
@@ -85,6 +95,7 @@ struct vx_lm {
   PersistStack bp;
   bool bp_on = true;
   bool bt_persist = false;  // the captured batch step uses it
+  const LmSampling* sampling = nullptr;  // the batched head draws by these instead of picking the largest
   cudaGraphExec_t step_exec = nullptr;
   unsigned long long step_kernels = 0;
   // persistent decode step (one launch per token), when the shape allows it
@@ -379,8 +390,8 @@ int ensure_batch(vx_lm* lm) {
   return VX_OK;
 }
 
-// Greedy head for B rows: final norm (kept as the hidden the DiT consumes), logits over the
-// tied embedding, per-row argmax -> token and next input embedding, then step (and position).
+// Head for B rows (greedy, or sampling where lm->sampling is set): final norm (kept as the hidden the DiT consumes), logits over the
+// tied embedding, per-row pick -> token and next input embedding, then step (and position).
 int enqueue_batch_head(vx_lm* lm, int B, cudaStream_t st, bool advance_pos, bool normed = false) {
   vx_ctx* ctx = lm->ctx;
   const int H = lm->H;
@@ -389,8 +400,15 @@ int enqueue_batch_head(vx_lm* lm, int B, cudaStream_t st, bool advance_pos, bool
                                          lm->bhid, st));
   int rc = linear(ctx, &lm->ws, lm->bhid, H, B, lm->V, H, lm->embed, nullptr, nullptr, 1.f, lm->blogits, lm->V, st);
   if (rc) return rc;
-  VX_CUDA(ctx, launch_argmax_rows(lm->blogits, B, lm->V, lm->d_step, lm->btokens, lm->max_batch, lm->embed, H,
-                                  lm->emb_scale, lm->bx, st));
+  if (const LmSampling* sp = lm->sampling) {
+    VX_CUDA(ctx, launch_sample(lm->blogits, lm->V, B, lm->V, sp->u, lm->d_step, sp->temperature, sp->top_k, sp->top_p,
+                               sp->min_p, sp->ids, nullptr, st));
+    VX_CUDA(ctx, launch_take_ids(sp->ids, B, lm->V, lm->d_step, lm->btokens, lm->max_batch, lm->embed, H, lm->emb_scale,
+                                 lm->bx, st));
+  } else {
+    VX_CUDA(ctx, launch_argmax_rows(lm->blogits, B, lm->V, lm->d_step, lm->btokens, lm->max_batch, lm->embed, H,
+                                    lm->emb_scale, lm->bx, st));
+  }
   VX_CUDA(ctx, launch_advance(lm->d_pos, lm->d_step, advance_pos, st));
   return VX_OK;
 }
@@ -904,9 +922,10 @@ int lm_greedy_begin(vx_lm* lm, const int32_t* prompt_ids, int n_prompt, int n_st
   return VX_OK;
 }
 
-// Batched greedy start for B prompts of equal length (ids [B][n_prompt]): causal prefill of
-// all rows filling the cache rows 0..B-1, then the head picks each row's first id.
-int lm_batch_begin(vx_lm* lm, const int32_t* prompt_ids, int B, int n_prompt, int n_steps) {
+// Batched start for B prompts of equal length (ids [B][n_prompt]): causal prefill of all rows
+// filling the cache rows 0..B-1, then the head picks each row's first id (by `sampling`, if any).
+static int batch_begin(vx_lm* lm, const int32_t* prompt_ids, int B, int n_prompt, int n_steps,
+                       const LmSampling* sampling) {
   vx_ctx* ctx = lm->ctx;
   if (!lm->embed) return fail(ctx, VX_ERR_CONFIG, "greedy decode needs a vocabulary");
   if (B <= 0 || B > lm->max_batch) return fail(ctx, VX_ERR_SHAPE, "batch %d outside 1..%d", B, lm->max_batch);
@@ -938,11 +957,18 @@ int lm_batch_begin(vx_lm* lm, const int32_t* prompt_ids, int B, int n_prompt, in
   VX_CUDA(ctx, cudaMemcpy2DAsync(lm->bx, (size_t)lm->H * 4, lm->pf_x + (size_t)(n_prompt - 1) * lm->H,
                                  (size_t)n_prompt * lm->H * 4, (size_t)lm->H * 4, B, cudaMemcpyDeviceToDevice, st));
   VX_CUDA(ctx, cudaMemsetAsync(lm->d_step, 0, 4, st));
-  if ((rc = enqueue_batch_head(lm, B, st, false))) return rc;
+  lm->sampling = sampling;
+  rc = enqueue_batch_head(lm, B, st, false);
+  lm->sampling = nullptr;
+  if (rc) return rc;
   lm->pos_host = n_prompt;
   VX_CUDA(ctx, cudaMemcpyAsync(lm->d_pos, &lm->pos_host, 4, cudaMemcpyHostToDevice, st));
   lm->cur_len = n_prompt;
   return VX_OK;
+}
+
+int lm_batch_begin(vx_lm* lm, const int32_t* prompt_ids, int B, int n_prompt, int n_steps) {
+  return batch_begin(lm, prompt_ids, B, n_prompt, n_steps, nullptr);
 }
 
 // One graph-replayed batched decode step (B rows as at lm_batch_begin).
@@ -1038,6 +1064,57 @@ int vx_lm_greedy(vx_lm* lm, const int32_t* prompt_ids, int n_prompt, int n_steps
   cudaEventElapsedTime(&lm->t_decode_ms, lm->ev[1], lm->ev[2]);
   lm->cur_len = pos0 + n_steps;
   return VX_OK;
+}
+
+int vx_lm_sample(vx_lm* lm, const int32_t* prompt_ids, int B, int n_prompt, int n_steps, const float* u,
+                 const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                 int32_t* tokens_out) {
+  if (!lm || !prompt_ids || !u || !tokens_out || n_prompt <= 0 || n_steps < 0) return VX_ERR_ARG;
+  vx_ctx* ctx = lm->ctx;
+  if (B <= 0 || B > lm->max_batch || B > 128)
+    return fail(ctx, VX_ERR_SHAPE, "batch %d outside 1..%d", B, std::min(lm->max_batch, 128));
+  if (lm->V > (1 << 18)) return fail(ctx, VX_ERR_SHAPE, "sampling: vocabulary %d > 2^18", lm->V);
+  if (n_steps >= lm->max_length)
+    return fail(ctx, VX_ERR_KV_FULL, "KV cache is full: %d prompt + %d steps > %d", n_prompt, n_steps, lm->max_length);
+  DeviceGuard guard(ctx->device);
+  cudaStream_t st = ctx->stream;
+  // one block: the random numbers of every pick, the four settings, the ids of a step
+  const size_t picks = (size_t)(n_steps + 1) * B, words = picks + 5 * (size_t)B;
+  float* d = nullptr;
+  if (cudaMalloc(&d, words * 4) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ctx, VX_ERR_OOM, "sampling: allocation failed");
+  }
+  float* set = d + picks;
+  const void* host[4] = {temperature, top_k, top_p, min_p};
+  cudaError_t e = cudaMemcpyAsync(d, u, picks * 4, cudaMemcpyDefault, st);
+  for (int i = 0; i < 4 && e == cudaSuccess; ++i)
+    if (host[i]) e = cudaMemcpyAsync(set + (size_t)i * B, host[i], (size_t)B * 4, cudaMemcpyDefault, st);
+  int rc = e == cudaSuccess ? VX_OK : cuda_fail(ctx, e, "sampling: upload");
+  const LmSampling sp = {d, temperature ? set : nullptr, top_k ? reinterpret_cast<int32_t*>(set + B) : nullptr,
+                         top_p ? set + 2 * (size_t)B : nullptr, min_p ? set + 3 * (size_t)B : nullptr,
+                         reinterpret_cast<int32_t*>(set + 4 * (size_t)B)};
+  if (!rc) rc = batch_begin(lm, prompt_ids, B, n_prompt, n_steps, &sp);
+  for (int s = 0; s < n_steps && !rc; ++s) {
+    if (ctx->cancel.load(std::memory_order_relaxed)) {
+      rc = fail(ctx, VX_ERR_CANCELLED, "generation cancelled");
+      break;
+    }
+    lm->sampling = &sp;
+    rc = enqueue_batch_step(lm, B, st);
+    lm->sampling = nullptr;
+    lm->cur_len += 1;
+  }
+  if (!rc) {
+    // the device keeps [step][max_batch]; the caller gets [B][n_steps + 1]
+    for (int b = 0; b < B && e == cudaSuccess; ++b)
+      e = cudaMemcpy2DAsync(tokens_out + (size_t)b * (n_steps + 1), 4, lm->btokens + b, (size_t)lm->max_batch * 4, 4,
+                            n_steps + 1, cudaMemcpyDeviceToHost, st);
+    rc = e == cudaSuccess ? check_device_error(ctx) : cuda_fail(ctx, e, "sampling: download");
+  }
+  cudaStreamSynchronize(st);
+  cudaFree(d);
+  return rc;
 }
 
 int vx_lm_profile_decode_step(vx_lm* lm, int pos, float* kernel_us, int n) {

@@ -53,6 +53,14 @@ cudaError_t launch_rope_scatter(const float* qkv, int B, int S, int nh, int nkv,
                                 const int* pos_ptr = nullptr);
 cudaError_t launch_argmax_rows(const float* logits, int B, int V, const int* step, int* tokens, int ld_tokens,
                                const uint16_t* E, int H, float scale, float* next_x, cudaStream_t st);
+// tokens[*step * ld_tokens + b] = ids[b] and the row's next input embed(ids[b]) * scale (id 0's where
+// there is no id).
+cudaError_t launch_take_ids(const int* ids, int B, int V, const int* step, int* tokens, int ld_tokens,
+                            const uint16_t* E, int H, float scale, float* next_x, cudaStream_t st);
+// vx_sample without its checks; with `step`, u holds a row of numbers for each step of a loop.
+cudaError_t launch_sample(const float* logits, int64_t row_stride, int rows, int vocab, const float* u, const int* step,
+                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                          int32_t* ids, float* logprob, cudaStream_t st);
 cudaError_t launch_advance(int* pos, int* step, bool inc_pos, cudaStream_t st);
 cudaError_t launch_rope_apply(float* x, int B, int H, int S, int d, const float* cos, const float* sin,
                               cudaStream_t st);

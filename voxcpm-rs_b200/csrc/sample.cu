@@ -49,7 +49,9 @@ struct SampleArgs {
   const float* logits;
   long long ld;
   int rows, vocab, slice;
-  const float *u, *temperature;
+  const float* u;   // [rows], or with `step` a row of them for each step
+  const int* step;  // device step of a decode loop, or null
+  const float* temperature;
   const int* top_k;
   const float *top_p, *min_p;
   int* ids;
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   row.tab = s.tab;
   row.x = a.logits + (size_t)r * a.ld + row.lo;
   const float temp = a.temperature ? a.temperature[r] : 1.f, p = a.top_p ? a.top_p[r] : 1.f;
-  const float mp = a.min_p ? a.min_p[r] : 0.f, uf = a.u[r];
+  const float mp = a.min_p ? a.min_p[r] : 0.f, uf = a.u[(a.step ? (size_t)*a.step * a.rows : 0) + r];
   int k = a.top_k ? a.top_k[r] : 0;
 
   // the row, its largest and its smallest finite logit, and whether it holds a NaN
@@ -746,6 +748,29 @@ cudaError_t sample_configure() {
   return cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SP_SLICE * 4);
 }
 
+cudaError_t launch_sample(const float* logits, int64_t row_stride, int rows, int vocab, const float* u, const int* step,
+                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                          int32_t* ids, float* logprob, cudaStream_t st) {
+  if (rows <= 0 || vocab <= 0 || vocab > SP_MAX_VOCAB) return cudaErrorInvalidValue;
+  const SampleShape p = shape_of(rows, vocab);
+  SampleArgs a = {logits, row_stride, rows, vocab, (vocab + p.blocks - 1) / p.blocks, u, step, temperature, top_k,
+                  top_p, min_p, ids, logprob};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows * p.blocks);
+  cfg.blockDim = dim3(SP_THREADS);
+  cfg.dynamicSmemBytes = p.in_shared ? (size_t)a.slice * 4 : 0;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.blocks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  count_launch();
+  return p.in_shared ? cudaLaunchKernelEx(&cfg, sample_kernel<true>, a) : cudaLaunchKernelEx(&cfg, sample_kernel<false>, a);
+}
+
 }  // namespace vx
 
 using namespace vx;
@@ -760,23 +785,7 @@ extern "C" int vx_sample(vx_ctx* ctx, const float* logits, int64_t row_stride, i
   if (row_stride < vocab) return fail(ctx, VX_ERR_SHAPE, "sample: row stride below the vocabulary");
   if (rows == 0) return VX_OK;
   DeviceGuard guard(ctx->device);
-  const SampleShape p = shape_of(rows, vocab);
-  SampleArgs a = {logits, row_stride, rows, vocab, (vocab + p.blocks - 1) / p.blocks, u, temperature, top_k, top_p,
-                  min_p, ids, logprob};
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows * p.blocks);
-  cfg.blockDim = dim3(SP_THREADS);
-  cfg.dynamicSmemBytes = p.in_shared ? (size_t)a.slice * 4 : 0;
-  cfg.stream = pick_stream(ctx, stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.blocks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  count_launch();
-  VX_CUDA(ctx, p.in_shared ? cudaLaunchKernelEx(&cfg, sample_kernel<true>, a)
-                           : cudaLaunchKernelEx(&cfg, sample_kernel<false>, a));
+  VX_CUDA(ctx, launch_sample(logits, row_stride, rows, vocab, u, nullptr, temperature, top_k, top_p, min_p, ids, logprob,
+                             pick_stream(ctx, stream)));
   return VX_OK;
 }

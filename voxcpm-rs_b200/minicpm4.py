@@ -275,6 +275,21 @@ class MiniCpmModel:
         check(lib().vx_lm_greedy(self.h, ptr(ids), len(ids), n_steps, ptr(out)), self.ctx.h)
         return out
 
+    def sample(self, prompt_ids, n_steps, u, temperature=None, top_k=None, top_p=None, min_p=None):
+        """``greedy`` with drawn ids for a batch of prompts ``[B, n_prompt]``: ``u [n_steps + 1, B]``
+        are the random numbers of the picks, the settings one value for all rows or ``[B]``
+        (None: off; see ``sampling.sample``).  Returns ids ``[B, n_steps + 1]``."""
+        ids = np.ascontiguousarray(np.atleast_2d(prompt_ids), dtype=np.int32)
+        b, n = ids.shape
+        u = np.ascontiguousarray(u, np.float32)
+        if u.shape != (n_steps + 1, b):
+            raise _lib.VxError(_lib.VX_ERR_SHAPE, f"u: shape {(n_steps + 1, b)} is needed, got {u.shape}")
+        rows = [None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, dt), (b,)))
+                for v, dt in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        out = np.empty((b, n_steps + 1), np.int32)
+        check(lib().vx_lm_sample(self.h, ptr(ids), b, n, n_steps, ptr(u), *[ptr(v) for v in rows], ptr(out)), self.ctx.h)
+        return out
+
     def last_logits(self):
         out = np.empty(self.cfg.vocab_size, np.float32)
         check(lib().vx_lm_last_logits(self.h, ptr(out)), self.ctx.h)
