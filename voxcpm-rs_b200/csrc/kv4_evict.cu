@@ -61,9 +61,33 @@ __device__ __forceinline__ uint32_t warps_before(const uint32_t* n, int warp, ui
   return __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
 }
 
+// n pieces of a type from one place to another, dealt to the block's threads.
+template <class T, class Where>
+__device__ __forceinline__ void move_pieces(uint32_t n, int tid, Where where) {
+  constexpr int U = 4;
+  for (uint32_t p0 = tid; p0 < n; p0 += U * EV_THREADS) {
+    T x[U];
+    T* onto[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t p = p0 + u * EV_THREADS;
+      onto[u] = nullptr;
+      if (p < n) {
+        const T* from;
+        where(p, &from, &onto[u]);
+        x[u] = *from;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (onto[u]) *onto[u] = x[u];
+  }
+}
+
 template <int ITEMS>
 __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a) {
   extern __shared__ __align__(16) uint32_t list[];  // free slots from the front, movers from the back
+  uint32_t* to = list + EV_THREADS * ITEMS;         // the slots that this block's movers take
   __shared__ EvictShared s;
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
@@ -232,65 +256,46 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
   }
   hole0 -= h_r;
   const uint32_t mine = all >> 16;
-  // 16 lanes move a row, four rows at a time to have their loads in flight together
-  const int l16 = tid & 15, cb = a.d / 32, sb = a.d / 64;  // 16-byte pieces of a row's codes, words of its scales
-  const uint8_t* src_base;
-  uint8_t* dst_base;
-  int row_bytes, kind;  // 0: 16 bytes, 1: 4 bytes, 2: 8 bytes
-  if (l16 < 2 * cb) {
-    kind = 0, row_bytes = a.d / 2;
-    dst_base = (l16 < cb ? a.k_codes : a.v_codes) + (l16 % cb) * 16;
-    src_base = dst_base;
-  } else if (l16 < 2 * cb + 2 * sb) {
-    const int i = l16 - 2 * cb;
-    kind = 1, row_bytes = a.d / 16;
-    dst_base = (i < sb ? a.k_scales : a.v_scales) + (i % sb) * 4;
-    src_base = dst_base;
-  } else if (l16 == 14) {
-    kind = 1, row_bytes = 4;
-    src_base = reinterpret_cast<const uint8_t*>(a.weights);
-    dst_base = reinterpret_cast<uint8_t*>(a.weights_out);
-  } else if (l16 == 15) {
-    kind = 2, row_bytes = 8;
-    src_base = reinterpret_cast<const uint8_t*>(a.positions);
-    dst_base = reinterpret_cast<uint8_t*>(a.positions_out);
-  } else {
-    kind = 3, row_bytes = 0, src_base = nullptr, dst_base = nullptr;
+  // where each mover goes: the block that holds the g-th free slot is the last one whose first is not above g
+  uint32_t first_of[EV_MAX_CLUSTER];
+#pragma unroll
+  for (int r = 0; r < EV_MAX_CLUSTER; ++r) first_of[r] = r < C ? __shfl_sync(0xffffffffu, hole0, r) : 0xffffffffu;
+  for (uint32_t i = tid; i < mine; i += EV_THREADS) {
+    const uint32_t g = m0 + i;
+    int owner = 0;
+    uint32_t start = 0;
+#pragma unroll
+    for (int r = 1; r < EV_MAX_CLUSTER; ++r)
+      if (g >= first_of[r]) owner = r, start = first_of[r];
+    to[i] = cl.map_shared_rank(list, owner)[g - start];
   }
-  src_base += row0 * row_bytes;
-  dst_base += row0 * row_bytes;
-  constexpr int kRows = EV_THREADS / 16;
-  for (uint32_t i0 = tid >> 4; i0 < (mine + kRows - 1) / kRows * kRows; i0 += 4 * kRows) {
-    uint4 x[4];
-    uint32_t dst[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t i = i0 + u * kRows, g = m0 + i;
-      // block that holds the g-th free slot: the last one whose first is not above g
-      uint32_t owner = 0, start = 0;
-#pragma unroll
-      for (int r = 1; r < EV_MAX_CLUSTER; ++r) {
-        const uint32_t f = __shfl_sync(0xffffffffu, hole0, r);
-        if (r < C && g >= f) owner = r, start = f;
-      }
-      dst[u] = 0xffffffffu;
-      if (i < mine) {
-        dst[u] = cl.map_shared_rank(list, owner)[g - start];
-        const uint8_t* p = src_base + (size_t)list[kLast - i] * row_bytes;
-        if (kind == 0) x[u] = *reinterpret_cast<const uint4*>(p);
-        if (kind == 1) x[u].x = *reinterpret_cast<const uint32_t*>(p);
-        if (kind == 2) *reinterpret_cast<uint2*>(&x[u]) = *reinterpret_cast<const uint2*>(p);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (dst[u] != 0xffffffffu) {
-        uint8_t* p = dst_base + (size_t)dst[u] * row_bytes;
-        if (kind == 0) *reinterpret_cast<uint4*>(p) = x[u];
-        if (kind == 1) *reinterpret_cast<uint32_t*>(p) = x[u].x;
-        if (kind == 2) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(&x[u]);
-      }
-  }
+  __syncthreads();
+  // one kind of piece after the other, each with full warps and four loads of a thread in flight
+  auto src = [&](uint32_t i) { return row0 + list[kLast - i]; };
+  auto dst = [&](uint32_t i) { return row0 + to[i]; };
+  const int cb = a.d / 32, lg = a.d == 128 ? 2 : 1;  // 16-byte pieces of a row's codes: 4 or 2; words of its scales: 2 or 1
+  move_pieces<uint4>(mine << (lg + 1), tid, [&](uint32_t p, const uint4** from, uint4** onto) {
+    const uint32_t i = p >> (lg + 1), c = p & (2 * cb - 1);
+    uint8_t* base = c < (uint32_t)cb ? a.k_codes : a.v_codes;
+    const size_t off = (size_t)(c & (cb - 1)) * 16;
+    *from = reinterpret_cast<const uint4*>(base + src(i) * (a.d / 2) + off);
+    *onto = reinterpret_cast<uint4*>(base + dst(i) * (a.d / 2) + off);
+  });
+  move_pieces<uint32_t>(mine << lg, tid, [&](uint32_t p, const uint32_t** from, uint32_t** onto) {
+    const uint32_t i = p >> lg, c = p & ((1 << lg) - 1), words = 1u << (lg - 1);
+    uint8_t* base = c < words ? a.k_scales : a.v_scales;
+    const size_t off = (size_t)(c & (words - 1)) * 4;
+    *from = reinterpret_cast<const uint32_t*>(base + src(i) * (a.d / 16) + off);
+    *onto = reinterpret_cast<uint32_t*>(base + dst(i) * (a.d / 16) + off);
+  });
+  move_pieces<float>(mine, tid, [&](uint32_t i, const float** from, float** onto) {
+    *from = a.weights + src(i);
+    *onto = a.weights_out + dst(i);
+  });
+  move_pieces<int64_t>(mine, tid, [&](uint32_t i, const int64_t** from, int64_t** onto) {
+    *from = a.positions + src(i);
+    *onto = a.positions_out + dst(i);
+  });
   cl.sync();  // the lists are read by the other blocks
 }
 
@@ -306,15 +311,18 @@ void evict_shape(int units, int max_len, int* C, int* items) {
 
 template <int ITEMS>
 cudaError_t evict_launch(cudaLaunchConfig_t& cfg, const EvictArgs& a) {
-  cfg.dynamicSmemBytes = (size_t)EV_THREADS * ITEMS * 4;
+  cfg.dynamicSmemBytes = (size_t)EV_THREADS * ITEMS * 8;
   return cudaLaunchKernelEx(&cfg, kv4_evict_kernel<ITEMS>, a);
 }
 
 }  // namespace
 
 cudaError_t kv4_evict_configure() {
+  const cudaError_t e = cudaFuncSetAttribute(kv4_evict_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             EV_THREADS * 16 * 8);
+  if (e != cudaSuccess) return e;
   return cudaFuncSetAttribute(kv4_evict_kernel<EV_MAX_ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              EV_THREADS * EV_MAX_ITEMS * 4);
+                              EV_THREADS * EV_MAX_ITEMS * 8);
 }
 
 }  // namespace vx

@@ -11,7 +11,7 @@ import ctypes as C
 
 from . import _lib
 from ._lib import VX_ERR_ARG, VX_ERR_SHAPE, VxError, check, lib
-from .minicpm4 import Context, _torch, raw_stream
+from .minicpm4 import Context, _torch
 
 
 def _refuse(code, msg):
@@ -74,25 +74,23 @@ class Kv4Cache:
         self._ref = C.addressof(self._c)
         self._lens_shape = torch.Size((b,))
         self._plans = {}
+        # what every call needs, looked up once: a call of a decode loop is a few microseconds of host time
+        self._f32, self._i32, self._empty = torch.float32, torch.int32, torch.empty
+        self._L, self._raw_stream = lib(), torch._C._cuda_getCurrentRawStream
 
     def _ints(self, t, what):
         if t is None:
             return None
-        _need(t, what, _torch().int32, self._lens_shape, self._index)
+        if t.dtype is not self._i32 or t.get_device() != self._index or t.shape != self._lens_shape or not t.is_contiguous():
+            _need(t, what, self._i32, self._lens_shape, self._index)
         return t.data_ptr()
-
-    def _run(self, fn, *args):
-        """One call of the library on the current stream of the cache's device."""
-        rc = fn(self.ctx.h, self._ref, *args, raw_stream(self._index))
-        if rc:
-            check(rc, self.ctx.h)
 
     def append(self, k, v, start, counts=None, first_position=None):
         """Quantise the rows of new tokens into the cache: ``k``, ``v`` f32 ``[B, S, nkv, d]``, the
         last two dims dense (views into a fused projection will do), token ``i < counts[b]`` into
         slot ``start[b] + i``.  Their weights become 0 and their positions
         ``first_position[b] + i`` (the slot without it)."""
-        f32 = _torch().float32
+        f32 = self._f32
         s = k.shape[1] if k.dim() == 4 else -1
         for t, what in ((k, "k"), (v, "v")):
             if t.shape != (self.batch, s, self.n_kv_heads, self.head_dim):
@@ -105,18 +103,22 @@ class Kv4Cache:
         st = k.stride()
         if st != v.stride() or st[3] != 1 or (st[2] != self.head_dim and self.n_kv_heads != 1):
             _refuse(VX_ERR_ARG, "k and v: dense heads and the same strides are needed")
-        self._run(lib().vx_kv4_append, k.data_ptr(), v.data_ptr(), st[0], st[1], s, self._ints(start, "start"),
-                  self._ints(counts, "counts"), self._ints(first_position, "first_position"))
+        rc = self._L.vx_kv4_append(self.ctx.h, self._ref, k.data_ptr(), v.data_ptr(), st[0], st[1], s,
+                                   self._ints(start, "start"), self._ints(counts, "counts"),
+                                   self._ints(first_position, "first_position"), self._raw_stream(self._index))
+        if rc:
+            check(rc, self.ctx.h)
 
     def read(self, n, start=None, counts=None):
         """The values of rows ``start[b] + i`` (``i < counts[b] <= n``; zeros behind them) as
         ``k, v`` f32 ``[B, nkv, n, d]``."""
-        torch = _torch()
         shape = (self.batch, self.n_kv_heads, n, self.head_dim)
-        k, v = torch.empty(shape, device=self.device), torch.empty(shape, device=self.device)
+        k, v = self._empty(shape, device=self.device), self._empty(shape, device=self.device)
         if n:
-            self._run(lib().vx_kv4_read, n, self._ints(start, "start"), self._ints(counts, "counts"), k.data_ptr(),
-                      v.data_ptr())
+            rc = self._L.vx_kv4_read(self.ctx.h, self._ref, n, self._ints(start, "start"), self._ints(counts, "counts"),
+                                     k.data_ptr(), v.data_ptr(), self._raw_stream(self._index))
+            if rc:
+                check(rc, self.ctx.h)
         return k, v
 
     def attend(self, q, lens, max_len=None, track=False, scale=None):
@@ -124,23 +126,25 @@ class Kv4Cache:
         strided) over its first ``lens[b]`` rows; ``lens[b] <= max_len`` (default the capacity; the
         work is split for that length).  Returns ``[B, nh * d]``.  With ``track`` the rows'
         ``weights`` grow by the probabilities that they received."""
-        torch = _torch()
-        if q.dtype is not torch.float32 or q.get_device() != self._index:
+        if q.dtype is not self._f32 or q.get_device() != self._index:
             _refuse(VX_ERR_ARG, f"q: f32 on {self.device} is needed, got {q.dtype} on {q.device}")
-        if q.dim() != 2 or q.shape[0] != self.batch or q.shape[1] % self.head_dim or q.stride(1) != 1:
-            _refuse(VX_ERR_SHAPE, f"q: dense rows [{self.batch}, nh * {self.head_dim}] are needed, got {tuple(q.shape)}")
+        batch, d = self.batch, self.head_dim
+        if q.dim() != 2 or q.shape[0] != batch or q.shape[1] % d or q.stride(1) != 1:
+            _refuse(VX_ERR_SHAPE, f"q: dense rows [{batch}, nh * {d}] are needed, got {tuple(q.shape)}")
         width = q.shape[1]
-        nh = width // self.head_dim
         n = self.capacity if max_len is None else max_len
-        key = (nh, n, bool(track))
+        key = (width // d, n, bool(track))
         need = self._plans.get(key)
         if need is None:
-            need = self._plans[key] = lib().vx_kv4_attend_workspace(self._ref, *key)
-        out = torch.empty((self.batch, width), device=self.device)
-        ws = torch.empty(need, device=self.device, dtype=torch.uint8) if need else None
-        self._run(lib().vx_kv4_attend, q.data_ptr(), q.stride(0) if self.batch > 1 else width, nh,
-                  self._ints(lens, "lens"), n, self.head_dim ** -0.5 if scale is None else scale, track,
-                  out.data_ptr(), width, None if ws is None else ws.data_ptr(), need)
+            need = self._plans[key] = self._L.vx_kv4_attend_workspace(self._ref, *key)
+        out = self._empty((batch, width), device=self.device)
+        ws = self._empty(need, device=self.device, dtype=_torch().uint8) if need else None
+        rc = self._L.vx_kv4_attend(self.ctx.h, self._ref, q.data_ptr(), q.stride(0) if batch > 1 else width, width // d,
+                                   self._ints(lens, "lens"), n, d ** -0.5 if scale is None else scale, track,
+                                   out.data_ptr(), width, None if ws is None else ws.data_ptr(), need,
+                                   self._raw_stream(self._index))
+        if rc:
+            check(rc, self.ctx.h)
         return out
 
     def evict(self, lens, seen, keep, sink=0, recent=0, max_len=None, weights_out=None, positions_out=None):
@@ -157,7 +161,9 @@ class Kv4Cache:
         _need(wo, "weights_out", torch.float32, self.weights.shape, self._index)
         _need(po, "positions_out", torch.int64, self.positions.shape, self._index)
         out = torch.empty(self._lens_shape, device=self.device, dtype=torch.int32)
-        self._run(lib().vx_kv4_evict, self._ints(lens, "lens"), self._ints(seen, "seen"),
-                  self.capacity if max_len is None else max_len, keep, sink, recent, wo.data_ptr(), po.data_ptr(),
-                  out.data_ptr())
+        rc = self._L.vx_kv4_evict(self.ctx.h, self._ref, self._ints(lens, "lens"), self._ints(seen, "seen"),
+                                  self.capacity if max_len is None else max_len, keep, sink, recent, wo.data_ptr(),
+                                  po.data_ptr(), out.data_ptr(), self._raw_stream(self._index))
+        if rc:
+            check(rc, self.ctx.h)
         return out
