@@ -488,17 +488,55 @@ __device__ __forceinline__ void head_stats(const AttendArgs& a, int unit, int r,
   *inv = 1.f / warp_sum(l * ex2(m - *M));
 }
 
-// The first units * 8 * slices blocks merge a head's columns (where there is more than one split),
-// D / slices of them: D / slices / 4 lanes read a split's, and the block's groups of lanes take
+// The first blocks merge the splits (where there is more than one).  Up to 32 of them: a warp for a
+// head and a block for a unit's 8, lane s has split s's maximum and sum.  More: a block merges D /
+// slices columns of a head, D / slices / 4 lanes read a split's and the block's groups of lanes take
 // other splits.  The blocks behind them add the probabilities of a run of positions of one KV head
 // to its weights, FIN_POS to a thread.
-constexpr int FIN_POS = 2;
+constexpr int FIN_POS = 4;
+constexpr int FIN_FEW = 32;
+
+template <int D>
+__device__ __forceinline__ void merge_few(const AttendArgs& a, int unit) {
+  constexpr int DPL = D / 32;
+  const int h = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hb = unit % a.nhb, g = (unit / a.nhb) % a.nkv, b = unit / (a.nhb * a.nkv);
+  const int n = seq_len(a, b);
+  if (n <= 0 || h >= HB || hb * HB + h >= a.nrep) return;
+  const int active = (n + a.chunk - 1) / a.chunk;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < active) ml = reinterpret_cast<const float2*>(a.part_ml)[((size_t)unit * a.nsplit + lane) * HB + h];
+  const float M = warp_max(ml.x), f = lane < active ? ex2(ml.x - M) : 0.f;
+  const float inv = 1.f / warp_sum(ml.y * f);
+  const float* po = a.part_o + ((size_t)unit * a.nsplit * HB + h) * D + lane * DPL;
+  float o[DPL] = {};
+#pragma unroll 8
+  for (int s = 0; s < active; ++s) {
+    const float fs = __shfl_sync(0xffffffffu, f, s);
+    const float2 x = *reinterpret_cast<const float2*>(po + (size_t)s * HB * D);
+    o[0] = fmaf(fs, x.x, o[0]);
+    o[1] = fmaf(fs, x.y, o[1]);
+    if constexpr (DPL == 4) {
+      const float2 y = *reinterpret_cast<const float2*>(po + (size_t)s * HB * D + 2);
+      o[2] = fmaf(fs, y.x, o[2]);
+      o[3] = fmaf(fs, y.y, o[3]);
+    }
+  }
+  float* out = a.out + (size_t)b * a.ldo + (size_t)(g * a.nrep + hb * HB + h) * D;
+#pragma unroll
+  for (int e = 0; e < DPL; e += 2)
+    *reinterpret_cast<float2*>(out + dim_of<D>(lane * DPL + e)) = make_float2(o[e] * inv, o[e + 1] * inv);
+}
 
 template <int D>
 __global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, int slices, int merge_blocks, int chunks) {
   extern __shared__ __align__(16) float4 acc[];  // one for each thread
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
+  if ((int)blockIdx.x < merge_blocks && a.nsplit <= FIN_FEW) {
+    merge_few<D>(a, blockIdx.x);
+    return;
+  }
   if ((int)blockIdx.x < merge_blocks) {
     const int slice = blockIdx.x % slices, r = blockIdx.x / slices % HB, unit = blockIdx.x / (slices * HB);
     const int hb = unit % a.nhb, g = (unit / a.nhb) % a.nkv, b = unit / (a.nhb * a.nkv);
@@ -730,8 +768,8 @@ int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* c, const float* q, int64_t q_stride
   // few units with many splits: more blocks to a head, and more groups of lanes in them
   const int slices = units <= 16 ? c->head_dim / 32 : 1;
   int threads = 256;
-  while (threads < 1024 && threads / (c->head_dim / 4 / slices) * 4 < p.nsplit) threads *= 2;
-  const int merge = p.nsplit > 1 ? units * HB * slices : 0, chunks = (max_len + FIN_POS * threads - 1) / (FIN_POS * threads);
+  while (p.nsplit > FIN_FEW && threads < 1024 && threads / (c->head_dim / 4 / slices) * 4 < p.nsplit) threads *= 2;
+  const int merge = p.nsplit == 1 ? 0 : p.nsplit <= FIN_FEW ? units : units * HB * slices, chunks = (max_len + FIN_POS * threads - 1) / (FIN_POS * threads);
   PdlLaunch pl(dim3(merge + (track ? a.B * a.nkv * chunks : 0)), dim3(threads), threads * sizeof(float4), st);
   count_launch();
   VX_CUDA(ctx, c->head_dim == 128 ? cudaLaunchKernelEx(&pl.cfg, kv4_finish_kernel<128>, a, slices, merge, chunks)

@@ -112,8 +112,7 @@ class Kv4Cache:
     def read(self, n, start=None, counts=None):
         """The values of rows ``start[b] + i`` (``i < counts[b] <= n``; zeros behind them) as
         ``k, v`` f32 ``[B, nkv, n, d]``."""
-        shape = (self.batch, self.n_kv_heads, n, self.head_dim)
-        k, v = self._empty(shape, device=self.device), self._empty(shape, device=self.device)
+        k, v = self._empty((2, self.batch, self.n_kv_heads, n, self.head_dim), device=self.device).unbind(0)
         if n:
             rc = self._L.vx_kv4_read(self.ctx.h, self._ref, n, self._ints(start, "start"), self._ints(counts, "counts"),
                                      k.data_ptr(), v.data_ptr(), self._raw_stream(self._index))
@@ -137,7 +136,7 @@ class Kv4Cache:
         need = self._plans.get(key)
         if need is None:
             need = self._plans[key] = self._L.vx_kv4_attend_workspace(self._ref, *key)
-        out = self._empty((batch, width), device=self.device)
+        out = q.new_empty((batch, width))
         ws = self._empty(need, device=self.device, dtype=_torch().uint8) if need else None
         rc = self._L.vx_kv4_attend(self.ctx.h, self._ref, q.data_ptr(), q.stride(0) if batch > 1 else width, width // d,
                                    self._ints(lens, "lens"), n, d ** -0.5 if scale is None else scale, track,
