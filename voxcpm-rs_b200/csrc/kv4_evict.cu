@@ -23,8 +23,8 @@ namespace vx {
 namespace {
 
 constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32;
-constexpr int EV_MAX_CLUSTER = 8;
-constexpr int EV_MAX_ITEMS = 32;  // keys of a thread
+constexpr int EV_MAX_CLUSTER = 16;  // above 8: not portable, but within one GPC of a B200
+constexpr int EV_MAX_ITEMS = 16;  // keys of a thread
 constexpr int EV_MAX_LEN = EV_THREADS * EV_MAX_CLUSTER * EV_MAX_ITEMS;  // 131072
 static_assert(EV_MAX_LEN == 131072, "the length that the header names");
 
@@ -299,11 +299,12 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
   cl.sync();  // the lists are read by the other blocks
 }
 
-// Blocks of a cluster and keys of a thread: as many blocks as keep about two on each SM, as few
-// keys as hold the longest sequence.
+// Blocks of a cluster and keys of a thread: as many blocks as keep about two on each SM (one, where
+// that takes clusters above 8, of which fewer fit a GPC: 16 units of 32768 rows 21 us at 8 and 36 at
+// 16, but 8 units of 125000 rows 83 and 59), as few keys as hold the longest sequence.
 void evict_shape(int units, int max_len, int* C, int* items) {
   *C = 1;
-  while (*C < EV_MAX_CLUSTER && max_len > EV_THREADS * 2 * *C && units * *C * 2 <= 296) *C *= 2;
+  while (*C < EV_MAX_CLUSTER && max_len > EV_THREADS * 2 * *C && units * *C * 2 <= (*C < 8 ? 296 : 148)) *C *= 2;
   while (max_len > EV_THREADS * EV_MAX_ITEMS * *C) *C *= 2;
   *items = 2;
   while (max_len > EV_THREADS * *items * *C) *items *= 2;
@@ -317,12 +318,20 @@ cudaError_t evict_launch(cudaLaunchConfig_t& cfg, const EvictArgs& a) {
 
 }  // namespace
 
-cudaError_t kv4_evict_configure() {
-  const cudaError_t e = cudaFuncSetAttribute(kv4_evict_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             EV_THREADS * 16 * 8);
+template <int ITEMS>
+static cudaError_t evict_allow() {
+  const cudaError_t e = cudaFuncSetAttribute(kv4_evict_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             EV_THREADS * ITEMS * 8);
   if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(kv4_evict_kernel<EV_MAX_ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              EV_THREADS * EV_MAX_ITEMS * 8);
+  return cudaFuncSetAttribute(kv4_evict_kernel<ITEMS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+
+cudaError_t kv4_evict_configure() {
+  cudaError_t e = evict_allow<2>();
+  if (e == cudaSuccess) e = evict_allow<4>();
+  if (e == cudaSuccess) e = evict_allow<8>();
+  if (e == cudaSuccess) e = evict_allow<16>();
+  return e;
 }
 
 }  // namespace vx
@@ -364,7 +373,6 @@ extern "C" int vx_kv4_evict(vx_ctx* ctx, const vx_kv4* c, const int32_t* lens, c
   VX_CUDA(ctx, items == 2    ? evict_launch<2>(cfg, a)
                : items == 4  ? evict_launch<4>(cfg, a)
                : items == 8  ? evict_launch<8>(cfg, a)
-               : items == 16 ? evict_launch<16>(cfg, a)
-                             : evict_launch<32>(cfg, a));
+                             : evict_launch<16>(cfg, a));
   return VX_OK;
 }
