@@ -27,6 +27,7 @@ constexpr int EV_MAX_CLUSTER = 16;  // above 8: not portable, but within one GPC
 constexpr int EV_MAX_ITEMS = 16;  // keys of a thread
 constexpr int EV_MAX_LEN = EV_THREADS * EV_MAX_CLUSTER * EV_MAX_ITEMS;  // 131072
 static_assert(EV_MAX_LEN == 131072, "the length that the header names");
+static_assert(EV_MAX_CLUSTER == 16, "the halves of the unrolled sums");
 
 struct EvictArgs {
   uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
@@ -140,8 +141,12 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
     if (tid < 256) {
       uint32_t t = 0;
 #pragma unroll
-      for (int r = 0; r < EV_MAX_CLUSTER; ++r)  // unrolled: one round trip for all blocks
+      for (int r = 0; r < 8; ++r)  // unrolled: one round trip for eight blocks
         if (r < C) t += cl.map_shared_rank(h, r)[tid];
+      if (C > 8) {
+#pragma unroll
+        for (int r = 8; r < 16; ++r) t += cl.map_shared_rank(h, r)[tid];
+      }
       s.tot[tid] = t;
     }
     __syncthreads();
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
     uint32_t start = 0;
 #pragma unroll
     for (int r = 1; r < EV_MAX_CLUSTER; ++r)
-      if (g >= first_of[r]) owner = r, start = first_of[r];
+      if (r < C && g >= first_of[r]) owner = r, start = first_of[r];
     to[i] = cl.map_shared_rank(list, owner)[g - start];
   }
   __syncthreads();
