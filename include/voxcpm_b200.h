@@ -209,7 +209,9 @@ int vx_kv4_read(vx_ctx* ctx, const vx_kv4* cache, int n, const int32_t* start, c
 /* Attention of one query token per sequence over its first lens[b] rows (as
  * vx_attention_decode over an f32 cache): q [batch] rows of nh * head_dim f32, q_stride
  * elements apart (16-byte aligned), query head h on KV head h / (nh / n_kv_heads); out likewise.
- * 0 <= lens[b] <= max_len; a sequence of length 0 gives zeros.  With track every row's weight
+ * 0 <= lens[b] <= max_len; a sequence of length 0 gives zeros, a query head that is not finite
+ * NaN.  Values are f32 throughout: products of the cached values are exact, and sums are f32;
+ * track does not change the output.  With track every row's weight
  * grows by the probabilities that it received from the query heads of its KV head.  The
  * workspace (16-byte aligned, vx_kv4_attend_workspace bytes, may be NULL for 0) is this call's
  * alone until it has run: calls and captured graphs that may overlap need one each. */

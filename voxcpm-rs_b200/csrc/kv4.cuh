@@ -71,8 +71,12 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t b) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
 }
 
-__device__ __forceinline__ float h2_lo(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)(h & 0xffff))); }
-__device__ __forceinline__ float h2_hi(uint32_t h) { return __half2float(__ushort_as_half((unsigned short)(h >> 16))); }
+__device__ __forceinline__ float h2_lo(uint32_t h) {
+  return __half2float(__ushort_as_half((unsigned short)(h & 0xffff)));
+}
+__device__ __forceinline__ float h2_hi(uint32_t h) {
+  return __half2float(__ushort_as_half((unsigned short)(h >> 16)));
+}
 
 // log2(e): scores are kept in base 2, so that a probability is one ex2
 constexpr float KV4_LOG2E = 1.4426950408889634f;

@@ -7,6 +7,15 @@
 // through distributed shared memory and has its scores there for `track`: one launch, no
 // workspace.  More splits leave them in the workspace, and kv4_finish_kernel joins them and turns
 // the scores that a tracking call left there into weights.
+//
+// What bounds it.  A position costs 144 bytes (d = 128) and 4 * 8 * 128 flops for 8 query heads, so HBM
+// is the floor; but the products need every value as f16, twice (a query and a probability have two
+// terms), and an SM does that for 16 positions in about 165 clocks, where HBM would allow 100: 32
+// tensor instructions (64 clocks alone), 64 conversions and 64 multiplications by scales, which share
+// the issue slots and, measured with nothing else around them, take 103 clocks together.  Long
+// batches run at 3.9 TB/s (64 sequences of 32768 rows: 153 us; floor 94); short ones are bound by
+// latency: launch, first tile, merge (one sequence of 64 rows 4.5 us, of 1001 rows in a cluster of
+// 8 splits 5.9 us).
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -529,7 +538,8 @@ __device__ __forceinline__ void merge_few(const AttendArgs& a, int unit) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, int slices, int merge_blocks, int chunks) {
+__global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, int slices, int merge_blocks,
+                                                          int chunks) {
   extern __shared__ __align__(16) float4 acc[];  // one for each thread
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
@@ -638,18 +648,27 @@ AttendPlan plan_of(const vx_kv4* c, int nh, int max_len, int track) {
   const int nrep = nh / c->n_kv_heads;
   p.nhb = (nrep + HB - 1) / HB;
   const long long units = (long long)c->batch * c->n_kv_heads * p.nhb;
-  // short sequences: the most splits, as long as all blocks are on the GPU at once (four to an SM)
-  auto chunk_of = [&](int splits) { return std::max(1, (max_len + splits * kLeast - 1) / (splits * kLeast)) * kLeast; };
+  // Short sequences: the most splits, as long as all blocks are on the GPU at once, four to an SM
+  // (8 sequences of 1024 rows: 8 splits in a cluster 7.0 us, through the workspace 7.1 us and one
+  // launch more, 1 split of 1024 rows 10.5 us).
+  auto chunk_of = [&](int splits) {
+    const long long run = (long long)splits * kLeast;
+    return std::max(1ll, (max_len + run - 1) / run) * kLeast;
+  };
   int splits = AT_MAX_CLUSTER;
-  while (splits > 1 && (units * splits > 148 * 4 || (splits / 2) * kLeast >= max_len) && chunk_of(splits / 2) <= AT_CLUSTER_CHUNK)
+  while (splits > 1 && (units * splits > 148 * 4 || (splits / 2) * kLeast >= max_len) &&
+         chunk_of(splits / 2) <= AT_CLUSTER_CHUNK)
     splits /= 2;
   // (several blocks of query heads would add to the same weights: not in a cluster)
   if (chunk_of(splits) <= AT_CLUSTER_CHUNK && p.nhb == 1) {
     p.cluster = true;
-    p.chunk = chunk_of(splits);
+    p.chunk = (int)chunk_of(splits);
     p.nsplit = splits;
     return p;
   }
+  // Long ones: two rounds of blocks, of 512 to 4096 positions (a block costs about 5 us next to its
+  // tiles; 64 sequences of 32768 rows: 512 positions 167 us, 4096 139 us; 32 ragged ones of up to
+  // 8191: 512 27 us, 4096 47 us; the sums of more splits than 256 cost more to merge than they save)
   long long chunk = (units * max_len + 148 * 8 - 1) / (148 * 8);
   const long long least = units * max_len <= 148 * 4 * kLeast ? kLeast : 512;
   chunk = std::min<long long>(4096, std::max(least, (chunk + kLeast - 1) / kLeast * kLeast));
@@ -661,7 +680,9 @@ AttendPlan plan_of(const vx_kv4* c, int nh, int max_len, int track) {
   return p;
 }
 
-constexpr size_t split_smem(int d) { return AT_WARPS * AT_STAGES * (d == 128 ? TileBytes<128>::all : TileBytes<64>::all); }
+constexpr size_t split_smem(int d) {
+  return AT_WARPS * AT_STAGES * (d == 128 ? TileBytes<128>::all : TileBytes<64>::all);
+}
 constexpr size_t cluster_smem(int d, int chunk, bool track) {
   return split_smem(d) + (track ? (size_t)chunk * HB * 4 : 0);
 }
@@ -769,7 +790,8 @@ int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* c, const float* q, int64_t q_stride
   const int slices = units <= 16 ? c->head_dim / 32 : 1;
   int threads = 256;
   while (p.nsplit > FIN_FEW && threads < 1024 && threads / (c->head_dim / 4 / slices) * 4 < p.nsplit) threads *= 2;
-  const int merge = p.nsplit == 1 ? 0 : p.nsplit <= FIN_FEW ? units : units * HB * slices, chunks = (max_len + FIN_POS * threads - 1) / (FIN_POS * threads);
+  const int merge = p.nsplit == 1 ? 0 : p.nsplit <= FIN_FEW ? units : units * HB * slices;
+  const int chunks = (int)(((long long)max_len + FIN_POS * threads - 1) / (FIN_POS * threads));
   PdlLaunch pl(dim3(merge + (track ? a.B * a.nkv * chunks : 0)), dim3(threads), threads * sizeof(float4), st);
   count_launch();
   VX_CUDA(ctx, c->head_dim == 128 ? cudaLaunchKernelEx(&pl.cfg, kv4_finish_kernel<128>, a, slices, merge, chunks)

@@ -122,7 +122,7 @@ struct Row {
     return z > -31.5 ? exp_of(z) : 0;
   }
   __device__ __forceinline__ u64 exp_of(double z) const {
-    constexpr double kShift = 6755399441055744.0;                   // 1.5 * 2^52: a sum with it is rounded to an integer
+    constexpr double kShift = 6755399441055744.0;  // 1.5 * 2^52: a sum with it is rounded to an integer
     const double t = fma(z, 23.083120654223414215, kShift);         // 16 / ln 2
     const int n = __double2loint(t);
     const double r = fma(t - kShift, -0.043321698784996581839, z);  // ln 2 / 16; |r| <= 0.0217
@@ -449,7 +449,8 @@ __device__ u64 radix_border(cg::cluster_group& cl, Shared& s, const R& row, u64 
       for (int e = 0; e < 8; ++e) {
         v[e] = 0;
         for (int r = 0; r < C; ++r)
-          v[e] += (u64)cl.map_shared_rank(hi, r)[255 - lane * 8 - e] << 32 | cl.map_shared_rank(lo, r)[255 - lane * 8 - e];
+          v[e] += (u64)cl.map_shared_rank(hi, r)[255 - lane * 8 - e] << 32 |
+                  cl.map_shared_rank(lo, r)[255 - lane * 8 - e];
         sum += v[e];
       }
       const u64 incl = warp_scan64(sum);
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   row.inv_t = greedy ? 1.0 : 1.0 / (double)temp;
   row.floor_ = -INFINITY;
   if (hi < INFINITY && row.inv_t > 1e-30 && row.inv_t < 1e30) {
-    const float f = (float)(row.lmax_d - 32.0 / row.inv_t);  // z of it lies below -31.5 if hi - f is 32 T, to a rounding
+    const float f = (float)(row.lmax_d - 32.0 / row.inv_t);
     if (f > -INFINITY && ((double)f - row.lmax_d) * row.inv_t < -31.5) row.floor_ = f;
   }
   if (greedy) k = 1;
@@ -768,7 +769,8 @@ cudaError_t launch_sample(const float* logits, int64_t row_stride, int rows, int
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   count_launch();
-  return p.in_shared ? cudaLaunchKernelEx(&cfg, sample_kernel<true>, a) : cudaLaunchKernelEx(&cfg, sample_kernel<false>, a);
+  return p.in_shared ? cudaLaunchKernelEx(&cfg, sample_kernel<true>, a)
+                     : cudaLaunchKernelEx(&cfg, sample_kernel<false>, a);
 }
 
 }  // namespace vx

@@ -81,7 +81,8 @@ class Kv4Cache:
     def _ints(self, t, what):
         if t is None:
             return None
-        if t.dtype is not self._i32 or t.get_device() != self._index or t.shape != self._lens_shape or not t.is_contiguous():
+        if (t.dtype is not self._i32 or t.get_device() != self._index or t.shape != self._lens_shape
+                or not t.is_contiguous()):
             _need(t, what, self._i32, self._lens_shape, self._index)
         return t.data_ptr()
 
