@@ -109,3 +109,30 @@ def test_sample_follows_the_distribution(ctx):
     p /= p.sum()
     assert np.abs(np.bincount(ids, minlength=V) - n * p).max() <= 1.5
     assert np.all(np.diff(ids) >= 0)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(k=1), dict(k=700), dict(k=15000), dict(p=0.3), dict(p=0.97), dict(p=0.9, mp=0.1),
+                                dict(k=2000, p=0.5), dict(T=0.05, p=0.8), dict(T=30.0, p=0.5), dict(T=1e35, p=0.5)])
+def test_sample_many_rows(ctx, kw):
+    """The form for many rows (read from L2): rows where the list is too short, the border lies at a
+    bucket's end, or nothing is ordinary.  20 copies of 8 rows give the same ids."""
+    rng = np.random.default_rng(11)
+    V = 20011
+    base = (rng.standard_normal(V) * 2.5).astype(np.float32)
+    peaks = base.copy()
+    peaks[rng.integers(0, V, 6)] += 14
+    masked = np.where(rng.random(V) < 0.9, -np.inf, base).astype(np.float32)
+    lowest = np.where(rng.random(V) < 0.5, np.finfo(np.float32).min, base).astype(np.float32)
+    two = rng.integers(0, 2, V).astype(np.float32)
+    pinf = base.copy()
+    pinf[[3, 19999]] = np.inf
+    near = (np.round(base * 4) / 4).astype(np.float32)
+    rows = np.stack([base, peaks, masked, lowest, two, pinf, near, np.zeros(V, np.float32)])
+    from voxcpm_rs_b200.sampling import sample
+    args = {n: kw.get(s) for n, s in (("temperature", "T"), ("top_k", "k"), ("top_p", "p"), ("min_p", "mp"))}
+    full = {n: None if v is None else _cuda(np.full(160, v, np.int32 if n == "top_k" else np.float32)) for n, v in args.items()}
+    for u in (0.0, 0.4321, 0.99):
+        want = [osm.sample_row(r, np.float32(u), np.float32(kw.get("T", 1.0)), kw.get("k", 0), np.float32(kw.get("p", 1.0)),
+                               np.float32(kw.get("mp", 0.0)))[0] for r in rows]
+        ids = sample(ctx, _cuda(np.tile(rows, (20, 1))), _cuda(np.full(160, u, np.float32)), **full).cpu().numpy()
+        assert ids.reshape(20, 8).tolist() == [want] * 20, u

@@ -15,10 +15,12 @@
 // The draw takes the first token in index order whose running sum of staying weights exceeds
 // u * total: sums of each warp's part of the row, then one block walks the part that holds it.
 //
-// What bounds it: where every token needs its weight, instruction issue in two passes (about 45 and
-// 40 instructions of a warp for 32 tokens: 13 f64 operations, a table read, two 32-bit shared-memory
-// atomics, 3.7 clocks of an SM where one 64-bit atomic is a compare-and-swap loop of 30) and, for
-// few rows, the round trips between the blocks (each about half a microsecond; six of them).
+// What bounds it: with many rows of which every token needs its weight, instruction issue in the pass
+// that computes it (13 f64 operations and a table read for each token) and the shared-memory atomics of
+// the counting pass before (256 rows of 151643 tokens 240 us, where reading them takes 24); with few
+// rows the round trips between the blocks (each about half a microsecond; six of them; one row of
+// 73448 tokens 16 us).  A 64-bit sum takes two 32-bit atomics, 3.7 clocks of an SM for 32 tokens, where
+// one 64-bit atomic is a compare-and-swap loop of 30.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -89,8 +91,10 @@ struct SampleShared {
   float kept[kWarps][64];               // logits whose weights a warp has yet to sum
   uint32_t part_lo[kWarps], part_hi[kWarps];  // the sum of each warp's part of the row
   u64 coarse[kCoarse];
-  u64 warp64[kWarps];
+  u64 warp64[kWarps], warp_sure[kWarps];
   u64 total, above, border;
+  u64 block_sum, run;  // of the draw: staying weight of this block, and before the part that holds the token
+  float into;  // how far into its bucket find_bucket's border lies
   uint32_t warp32[kWarps];
   float fmax, fmin;
   int bad, bucket, n;
@@ -171,51 +175,67 @@ struct Buckets {
   __device__ __forceinline__ int operator()(float l) const { return (int)place(l); }
 };
 
+// What find_bucket adds up: tokens, their weights (PLAIN: in a row without special cases), or, in such a
+// row, for each token the weight at the middle of its bucket, which needs no exponential of its own.
+enum { SP_TOKENS, SP_WEIGHTS, SP_PLAIN, SP_MIDDLES };
+
 // The histogram over the cluster of value(l, index) and the bucket in which the running sum from
 // the largest logit on reaches need(total): s.bucket, s.above (the sum before it), s.total.  Every
 // block finds the same.
-template <bool wide, class Shared, class R, class Value, class Need>
-__device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, const Buckets<Shared>& bucket, bool plain,
-                            Value value, Need need) {
+template <int KIND, class Shared, class R, class Value, class Need>
+__device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, const Buckets<Shared>& bucket, Value value,
+                            Need need) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, C = (int)cl.num_blocks();
   for (int i = tid; i < Shared::kBuckets; i += Shared::kThreads) s.hist.lo[i] = s.hist.hi[i] = 0;
   __syncthreads();
-  constexpr int U = 4;  // logits of a thread whose weights are computed together
-  int j0 = tid;
-  if (plain) {  // `per` is finite and no logit above the floor lies behind the last bucket
-    for (; j0 - tid + U * Shared::kThreads <= row.cnt; j0 += U * Shared::kThreads) {
-      float l[U];
-      u64 v[U];
+  constexpr int U = 4;  // logits of a thread that are on their way together
+  // middles: the few tokens of weight above exp(-6) are added exactly, a large one's middle may be half
+  // a percent of all off
+  const int exact = KIND == SP_MIDDLES ? (int)fminf((float)(6.0 / row.inv_t) * bucket.per, (float)Shared::kBuckets) : 0;
+  for (int j0 = tid; j0 < row.cnt; j0 += U * Shared::kThreads) {
+    float l[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) l[i] = row.at(j0 + i * Shared::kThreads);
+    for (int i = 0; i < U; ++i) l[i] = j0 + i * Shared::kThreads < row.cnt ? row.at(j0 + i * Shared::kThreads) : -INFINITY;
+    // plain rows: `per` is finite and no logit above the floor lies behind the last bucket
+    if constexpr (KIND == SP_MIDDLES) {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (l[i] > row.floor_) {
+          const int at = (int)((bucket.lmax - l[i]) * bucket.per);
+          if (at >= exact)
+            atomicAdd(&s.hist.lo[at], 1u);
+          else
+            add64(&s.hist.lo[at], &s.hist.hi[at], row.weight(l[i]));
+        }
+    } else if constexpr (KIND == SP_PLAIN) {
+      u64 v[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) v[i] = row.exp_of(((double)fmaxf(l[i], row.floor_) - row.lmax_d) * row.inv_t);
 #pragma unroll
       for (int i = 0; i < U; ++i)
         if (l[i] > row.floor_) {
-          const int b = (int)((bucket.lmax - l[i]) * bucket.per);
-          add64(&s.hist.lo[b], &s.hist.hi[b], v[i]);
+          const int at = (int)((bucket.lmax - l[i]) * bucket.per);
+          add64(&s.hist.lo[at], &s.hist.hi[at], v[i]);
         }
+    } else {
+      u64 v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[i] = l[i] > -INFINITY ? value(l[i], row.lo + j0 + i * Shared::kThreads) : 0;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int at = bucket(l[i]);
+        if (v[i] && KIND == SP_WEIGHTS) add64(&s.hist.lo[at], &s.hist.hi[at], v[i]);
+        if (v[i] && KIND == SP_TOKENS) atomicAdd(&s.hist.lo[at], (uint32_t)v[i]);
+      }
     }
   }
-  for (; j0 < row.cnt; j0 += U * Shared::kThreads) {
-    u64 v[U];
-    int at[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int j = j0 + i * Shared::kThreads;
-      const float l = j < row.cnt ? row.at(j) : -INFINITY;
-      v[i] = l > -INFINITY ? value(l, row.lo + j) : 0;
-      at[i] = bucket(l);
+  if constexpr (KIND == SP_MIDDLES) {
+    __syncthreads();
+    for (int i = exact + tid; i < Shared::kBuckets; i += Shared::kThreads) {
+      const u64 v = s.hist.lo[i] ? s.hist.lo[i] * row.exp_of(-(i + 0.5) / bucket.per * row.inv_t) : 0;
+      s.hist.lo[i] = (uint32_t)v;
+      s.hist.hi[i] = (uint32_t)(v >> 32);
     }
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (v[i]) {
-        if (wide)
-          add64(&s.hist.lo[at[i]], &s.hist.hi[at[i]], v[i]);
-        else
-          atomicAdd(&s.hist.lo[at[i]], (uint32_t)v[i]);
-      }
   }
   __syncthreads();
   for (int c = warp; c < Shared::kCoarse; c += Shared::kWarps) {
@@ -257,8 +277,9 @@ __device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, cons
     const u64 fi = warp_scan64(f) + above;
     const uint32_t fh = __ballot_sync(0xffffffffu, fi >= want);
     const int b = fh ? __ffs(fh) - 1 : 31;
-    const u64 before = __shfl_sync(0xffffffffu, fi - f, b);
+    const u64 before = __shfl_sync(0xffffffffu, fi - f, b), own = __shfl_sync(0xffffffffu, f, b);
     if (lane == 0) {
+      s.into = (float)((double)(want - before) / (double)own);
       s.bucket = c * (Shared::kBuckets / Shared::kCoarse) + b;
       s.above = before;
       s.total = total;
@@ -354,6 +375,50 @@ __device__ u64 sum_kept(Shared& s, const R& row, int j0, int j1, u64 least, Keep
   add(lane < n, buf[lane]);
   __syncwarp();
   return warp_sum64(sum);
+}
+
+// A warp's sums over the logits j in [j0, j1) of a row without special cases, each weight computed
+// once: of all, of those before bucket `from`, and of the latter the weights of at least `least`.
+// Those in buckets [from, behind) go on the list.
+struct Sums {
+  u64 all, sure, kept;
+};
+template <class Shared, class R>
+__device__ Sums sum_all(Shared& s, const R& row, const Buckets<Shared>& bucket, int j0, int j1, float from, float behind,
+                        u64 least) {
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31;
+  Sums t = {0, 0, 0};
+  for (int j = j0 + lane; j - lane < j1; j += U * 32) {
+    float l[U], at[U];
+    u64 w[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) l[i] = j + 32 * i < j1 ? row.at(j + 32 * i) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      w[i] = row.exp_of(((double)fmaxf(l[i], row.floor_) - row.lmax_d) * row.inv_t);  // 0 at the floor
+      at[i] = (bucket.lmax - l[i]) * bucket.per;
+    }
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      t.all += w[i];
+      if (at[i] < from) {
+        t.sure += w[i];
+        if (w[i] >= least) t.kept += w[i];
+      }
+      some |= at[i] >= from && at[i] < behind;
+    }
+    if (__any_sync(0xffffffffu, some)) {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        append(s, at[i] >= from && at[i] < behind && l[i] > row.floor_, l[i], row.lo + j + 32 * i);
+    }
+  }
+  t.all = warp_sum64(t.all);
+  t.sure = warp_sum64(t.sure);
+  t.kept = warp_sum64(t.kept);
+  return t;
 }
 
 // ent[0, n) in descending order; entries differ from one another.  Long lists: bitonic; a thread has one pair
@@ -557,7 +622,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     Buckets<Shared> bucket = {hi, 0.f};
     const float range = fminf(hi - lo, 64.f * fmaxf(1.f, greedy ? 1.f : temp));
     bucket.per = range > 0.f ? (Shared::kBuckets - 1) / range : 0.f;
-    find_bucket<false>(cl, s, row, bucket, false, [](float, int) { return (u64)1; },
+    find_bucket<SP_TOKENS>(cl, s, row, bucket, [](float, int) { return (u64)1; },
                 [&](u64 total) { return total < (u64)k ? total : (u64)k; });
     const int last = s.bucket;
     const u64 want = s.total < (u64)k ? s.total : (u64)k;  // tokens of -infinity never stay
@@ -616,42 +681,22 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     Buckets<Shared> bucket = {hi, 0.f};
     const float range = fminf(hi - lo, (float)(32.1 / row.inv_t));  // beyond, no token has a weight
     bucket.per = range > 0.f ? (Shared::kBuckets - 1) / range : 0.f;
-    auto weight = [&](float l, int i) { return entry_of(l, i) >= first ? row.weight(l) : (u64)0; };
-    const bool plain = first == 0 && row.floor_ > -INFINITY && bucket.per < 1e30f;
-    if (first == 0)
-      find_bucket<true>(cl, s, row, bucket, plain, [&](float l, int) { return row.weight(l); }, need_of);
-    else
-      find_bucket<true>(cl, s, row, bucket, false, weight, need_of);
-    const float last = (float)s.bucket;
-    const u64 want = need_of(s.total), above = s.above;
-    // before the border's bucket all stay; the bucket's own go on the list
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    const float next = last + 1.f;
-    const u64 sure = plain ? sum_kept(s, row, w0, w1, least, [&](float l, int j) {
-      const float at = (bucket.lmax - l) * bucket.per;
-      append(s, l > row.floor_ && at >= last && at < next, l, row.lo + j);
-      return at < last && l >= low;
-    }) : sum_kept(s, row, w0, w1, least, [&](float l, int j) {
-      const float at = bucket.place(l);
-      const bool in = j < w1 && (first == 0 || entry_of(l, row.lo + j) >= first);
-      append(s, in && at >= last && at < next, l, row.lo + j);
-      return in && at < last && l >= low;
-    });
-    if (lane == 0) s.part_lo[warp] = (uint32_t)sure, s.part_hi[warp] = (uint32_t)(sure >> 32);
-    const int n = collect(cl, s);
-    if (n <= Shared::kList) {
+    // the border by the entries of block 0's list, of which the running sum before them is `above`; 0 if
+    // it is not among them
+    auto border_of_list = [&](int n, u64 above, u64 want) {
       if (rank == 0) {
         sort_list(s, n);
         for (int i = tid; i < n; i += THREADS) s.list.wt[i] = row.weight(logit_of(s.ent[i]));
         __syncthreads();
         scan_list(s, n, [&](int i) { return s.list.wt[i]; });
-        const int place = count_below(s, n, want - above);
-        if (tid == 0) s.border = s.ent[place];
+        const int place = above < want ? count_below(s, n, want - above) : n;
+        if (tid == 0) s.border = place < n ? s.ent[place] : 0;
       }
       cl.sync();
-      border = *cl.map_shared_rank(&s.border, 0);
-      // those of the list that stay and lie in this block join their warp's sum
+      return *cl.map_shared_rank(&s.border, 0);
+    };
+    // those of the list that stay and lie in this block join their warp's sum
+    auto add_list = [&](int n) {
       const int own = rank == 0 ? n : s.n;
       for (int i = tid; i < own; i += THREADS) {
         const u64 e = s.ent[i];
@@ -660,10 +705,71 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
         const u64 w = row.weight(logit_of(e));
         if (w && w >= least) add64(&s.part_lo[j / part], &s.part_hi[j / part], w);
       }
-      summed = true;
       __syncthreads();
-    } else {
-      border = radix_border(cl, s, row, want, weight);
+    };
+    const bool plain = first == 0 && row.floor_ > -INFINITY && bucket.per > 0.f && bucket.per < 1e30f;
+    if (!IN_SHARED && plain) {
+      // The bucket by middles, which may be off by one where the border lies near its end; then the
+      // exact sums and a list of the bucket and that neighbour, each token's weight computed once (256
+      // rows of 151643 tokens 288 -> 240 us; with few rows the longer list costs more than that saves).
+      find_bucket<SP_MIDDLES>(cl, s, row, bucket, [](float, int) { return (u64)0; }, need_of);
+      const float from = (float)max(0, s.bucket - (s.into < 0.25f)), behind = (float)(s.bucket + 1 + (s.into > 0.75f));
+      if (tid == 0) s.n = 0;
+      __syncthreads();
+      const Sums t = sum_all(s, row, bucket, w0, w1, from, behind, least);
+      if (lane == 0) {
+        s.warp64[warp] = t.all;
+        s.warp_sure[warp] = t.sure;
+        s.part_lo[warp] = (uint32_t)t.kept;
+        s.part_hi[warp] = (uint32_t)(t.kept >> 32);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const u64 all = warp_sum64(lane < kWarps ? s.warp64[lane] : 0);
+        const u64 sure = warp_sum64(lane < kWarps ? s.warp_sure[lane] : 0);
+        if (lane == 0) s.total = all, s.above = sure;
+      }
+      const int n = collect(cl, s);
+      const u64 total = warp_sum64(lane < C ? *cl.map_shared_rank(&s.total, lane) : 0);
+      const u64 sure = warp_sum64(lane < C ? *cl.map_shared_rank(&s.above, lane) : 0);
+      if (n > 0 && n <= Shared::kList) border = border_of_list(n, sure, need_of(total));
+      if (border) {
+        add_list(n);
+        summed = true;
+      } else {
+        cl.sync();  // the other blocks have read total, above and border
+      }
+    }
+    if (!summed) {
+      auto weight = [&](float l, int i) { return first == 0 || entry_of(l, i) >= first ? row.weight(l) : (u64)0; };
+      if (plain)
+        find_bucket<SP_PLAIN>(cl, s, row, bucket, [](float, int) { return (u64)0; }, need_of);
+      else
+        find_bucket<SP_WEIGHTS>(cl, s, row, bucket, weight, need_of);
+      const float last = (float)s.bucket, next = last + 1.f;
+      const u64 want = need_of(s.total), above = s.above;
+      // before the border's bucket all stay; the bucket's own go on the list
+      if (tid == 0) s.n = 0;
+      __syncthreads();
+      const u64 sure = plain ? sum_kept(s, row, w0, w1, least, [&](float l, int j) {
+        const float at = (bucket.lmax - l) * bucket.per;
+        append(s, l > row.floor_ && at >= last && at < next, l, row.lo + j);
+        return at < last && l >= low;
+      }) : sum_kept(s, row, w0, w1, least, [&](float l, int j) {
+        const float at = bucket.place(l);
+        const bool in = j < w1 && (first == 0 || entry_of(l, row.lo + j) >= first);
+        append(s, in && at >= last && at < next, l, row.lo + j);
+        return in && at < last && l >= low;
+      });
+      if (lane == 0) s.part_lo[warp] = (uint32_t)sure, s.part_hi[warp] = (uint32_t)(sure >> 32);
+      const int n = collect(cl, s);
+      if (n <= Shared::kList) {
+        border = border_of_list(n, above, want);
+        add_list(n);
+        summed = true;
+      } else {
+        border = radix_border(cl, s, row, want, weight);
+      }
     }
   }
 
@@ -686,10 +792,10 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     const u64 v = lane < kWarps ? s.warp64[lane] : 0;
     const u64 incl = warp_scan64(v);
     before = __shfl_sync(0xffffffffu, incl - v, warp);
-    if (tid == 31) s.total = incl;
+    if (tid == 31) s.block_sum = incl;
   }
   cl.sync();
-  const u64 block_sum = lane < C ? *cl.map_shared_rank(&s.total, lane) : 0;
+  const u64 block_sum = lane < C ? *cl.map_shared_rank(&s.block_sum, lane) : 0;
   const u64 block_incl = warp_scan64(block_sum);
   const u64 total = __shfl_sync(0xffffffffu, block_incl, 31), at = drawn(total);
   before += __shfl_sync(0xffffffffu, block_incl - block_sum, rank);
@@ -697,11 +803,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   __syncthreads();
   if (lane == 0 && before <= at && at < before + sum) {
     s.n = warp;
-    s.above = before;
+    s.run = before;
   }
   __syncthreads();
   if (s.n >= 0) {  // one block of the cluster: all its warps walk the part of that warp
-    u64 run = s.above;
+    u64 run = s.run;
     const int j0 = s.n * part, j1 = min(row.cnt, j0 + part);
     for (int j = j0 + tid; j - tid < j1; j += THREADS) {
       u64 w = j < j1 && stays(row.at(j), j) ? row.weight(row.at(j)) : 0;
@@ -733,7 +839,7 @@ constexpr int SP_SLICE = 32768;  // logits of a block in shared memory at most: 
 constexpr int SP_TWO = 18432;    // that leave room for two blocks on an SM
 // As many blocks of a row as there are SMs for (one row of 73448 tokens: 8 blocks 15 us, 2 blocks
 // 27 us; 64 rows: 4 blocks 38 us, 8 blocks 52 us).  256 rows of 151643 tokens: 2 blocks that read L2
-// 288 us, 8 with the row in shared memory 347 us.
+// 240 us (288 without the middles), 8 with the row in shared memory 347 us.
 SampleShape shape_of(int rows, int vocab) {
   SampleShape p = {1, true};
   while (p.blocks < SP_MAX_CLUSTER && vocab > 2048 * p.blocks && rows * p.blocks < 148) p.blocks *= 2;
