@@ -173,11 +173,11 @@ int vx_fsq(vx_ctx* ctx, const uint16_t* w_in, const float* b_in, const uint16_t*
  *   weights             [batch, n_kv_heads, capacity] f32 or NULL: the attention that each row
  *                       has received, summed (vx_kv4_attend with track)
  *   positions           [batch, n_kv_heads, capacity] int64 or NULL: the token position of each row
- * head_dim is 64 or 128, capacity a multiple of 32, codes and scales are 16-byte aligned.
+ * head_dim is 64 or 128, capacity a multiple of 32 (<= 2^30), codes and scales are 16-byte aligned.
  * How many rows of a sequence are filled is the caller's: device int32 arrays of `batch`
  * lengths, so that a captured graph can be replayed at other lengths.  Lengths outside their
  * range are found on the device: the sequence is left as it was (vx_kv4_attend: its output is
- * NaN) and the next vx_ctx_synchronize reports VX_ERR_ARG.  Calls that write a cache and calls
+ * NaN, vx_kv4_read: zeros, vx_kv4_evict: its length comes back unchanged) and the next vx_ctx_synchronize reports VX_ERR_ARG.  Calls that write a cache and calls
  * that read it are ordered by the caller (one stream, or events). */
 typedef struct {
   uint8_t* k_codes;
@@ -226,7 +226,7 @@ int vx_kv4_attend(vx_ctx* ctx, const vx_kv4* cache, const float* q, int64_t q_st
  * stay where they are; the i-th free slot there takes the i-th kept row behind it, with its
  * weight and position (attention does not depend on the order of rows).  weights_out and
  * positions_out [batch, n_kv_heads, capacity] receive the kept rows' (they may be the cache's
- * own; entries past the new length are left as they were); lens_out (not lens) receives
+ * own; entries past the new length are left as they were); lens_out (neither lens nor seen) receives
  * min(lens[b], keep). */
 int vx_kv4_evict(vx_ctx* ctx, const vx_kv4* cache, const int32_t* lens, const int32_t* seen, int max_len, int keep,
                  int sink, int recent, float* weights_out, int64_t* positions_out, int32_t* lens_out,
@@ -234,8 +234,8 @@ int vx_kv4_evict(vx_ctx* ctx, const vx_kv4* cache, const int32_t* lens, const in
 
 /* ----------------------------------------------------------------- sampling */
 
-/* One token id of each row of logits [rows, vocab] f32 (rows row_stride elements apart, vocab
- * <= 262144) by its own settings (device arrays of `rows`, NULL: off), where vx_lm_greedy picks
+/* One token id of each row of logits [rows, vocab] f32 (rows row_stride >= 0 elements apart, so
+ * that one row may serve many draws; vocab <= 262144) by its own settings (device arrays of `rows`, NULL: off), where vx_lm_greedy picks
  * the largest.  A token's weight is exp((l - lmax) / temperature), taken to 44 binary places;
  * temperature 0 is the greedy pick.  In the order of logits (descending, ties to the lowest id)
  *   top_k   the first k stay (k <= 0 or >= vocab: all)

@@ -358,3 +358,63 @@ def test_lengths_out_of_range_are_reported(ctx):
         assert lens.tolist() == [32, bad, 32]
         assert all(np.array_equal(p[1], q_[1]) for p, q_ in zip(before, _raw(c)))
         reported()
+
+
+def test_arguments_are_refused(ctx):
+    """Calls of the C ABI that its checks turn down: nothing is launched, the cache stays as it was."""
+    import ctypes as C
+    import torch
+    from voxcpm_rs_b200 import _lib
+    rng = np.random.default_rng(12)
+    c, _, _ = _filled(ctx, rng, 2, 2, 9632, 64)
+    L, before = _lib.lib(), _raw(c)
+    one, n = _i32([1, 1]), torch.zeros(2, device="cuda", dtype=torch.int32)
+    x, f = torch.zeros(1 << 16, device="cuda"), torch.zeros(2, 2, 9632, device="cuda")
+    p = lambda t, off=0: t.data_ptr() + off  # noqa: E731
+
+    def cache(**kw):
+        d = _lib.Kv4C()
+        C.memmove(C.addressof(d), c._ref, C.sizeof(d))
+        for name, v in kw.items():
+            setattr(d, name, v)
+        return d
+
+    def append(d, k=x, off=0, bs=128, ts=128, S=1, start=one):
+        return L.vx_kv4_append(ctx.h, C.addressof(d), p(k, off), p(x), bs, ts, S, start if start is None else p(start), None,
+                               None, None)
+
+    def attend(d, q_off=0, ldq=512, nh=8, lens=one, max_len=32, track=0, ldo=512, ws=None, ws_bytes=0):
+        return L.vx_kv4_attend(ctx.h, C.addressof(d), p(x, q_off), ldq, nh, p(lens), max_len, 1.0, track, p(x), ldo, ws,
+                               ws_bytes, None)
+
+    def evict(d, lens=one, seen=one, max_len=32, keep=8, sink=0, recent=0, out=n):
+        return L.vx_kv4_evict(ctx.h, C.addressof(d), p(lens), p(seen), max_len, keep, sink, recent, p(f), p(f), p(out), None)
+
+    good = cache()
+    A, S = _lib.VX_ERR_ARG, _lib.VX_ERR_SHAPE
+    bad = [(cache(head_dim=96), S), (cache(capacity=33), S), (cache(capacity=0), S), (cache(capacity=2 ** 30 + 32), S),
+           (cache(batch=0), S), (cache(n_kv_heads=0), S), (cache(n_kv_heads=32768), S), (cache(batch=40000), S),
+           (cache(k_codes=None), A), (cache(v_scales=c.v_scales.data_ptr() + 8), A)]
+    for d, code in bad:
+        assert [append(d), attend(d), evict(d)] == [code] * 3
+        assert L.vx_kv4_read(ctx.h, C.addressof(d), 1, None, None, p(x), p(x), None) == code
+    need = L.vx_kv4_attend_workspace(C.addressof(good), 8, 9632, 1)
+    ws = torch.empty(need, device="cuda", dtype=torch.uint8)
+    calls = [(append(good, off=4), A), (append(good, bs=130), A), (append(good, ts=2), A), (append(good, S=9633), S),
+             (append(good, S=-1), S), (append(good, start=None), A),
+             (L.vx_kv4_read(ctx.h, C.addressof(good), 9633, None, None, p(x), p(x), None), S),
+             (L.vx_kv4_read(ctx.h, C.addressof(good), -1, None, None, p(x), p(x), None), S),
+             (L.vx_kv4_read(ctx.h, C.addressof(good), 1, None, None, p(x, 8), p(x), None), A),
+             (attend(good, q_off=8), A), (attend(good, ldq=513), A), (attend(good, ldo=508), A), (attend(good, nh=0), S),
+             (attend(good, nh=3), S), (attend(good, nh=130), S), (attend(good, max_len=-1), S),
+             (attend(good, max_len=9633), S), (attend(cache(weights=None), track=1), A),
+             (attend(good, max_len=9632, track=1), A), (attend(good, max_len=9632, track=1, ws=p(ws), ws_bytes=need - 1), A),
+             (attend(good, max_len=9632, track=1, ws=p(ws, 8), ws_bytes=need), A),
+             (evict(cache(weights=None)), A), (evict(cache(positions=None)), A), (evict(good, lens=n), A),
+             (evict(good, seen=n), A), (evict(good, max_len=9633), S), (evict(good, max_len=-1), S),
+             (evict(good, keep=-1), S), (evict(good, sink=4, recent=5), S), (evict(good, sink=-1), S),
+             (evict(good, sink=2 ** 31 - 1, recent=2 ** 31 - 1), S)]
+    assert [got for got, _ in calls] == [code for _, code in calls]
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    assert all(np.array_equal(a, b) for a, b in zip(before, _raw(c))) and (f == 0).all() and (n == 0).all()

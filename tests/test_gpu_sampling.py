@@ -136,3 +136,21 @@ def test_sample_many_rows(ctx, kw):
                                np.float32(kw.get("mp", 0.0)))[0] for r in rows]
         ids = sample(ctx, _cuda(np.tile(rows, (20, 1))), _cuda(np.full(160, u, np.float32)), **full).cpu().numpy()
         assert ids.reshape(20, 8).tolist() == [want] * 20, u
+
+
+def test_sample_one_row_for_many_draws(ctx):
+    """An expanded row (stride 0) is read by every draw; a negative stride is refused."""
+    import torch
+    from voxcpm_rs_b200 import _lib
+    from voxcpm_rs_b200.sampling import sample
+    rng = np.random.default_rng(4)
+    x, u = _logits(rng, 1, 3001), rng.random(37).astype(np.float32)
+    t = _cuda(x)
+    ids = sample(ctx, t.expand(37, 3001), _cuda(u), top_p=_cuda(np.full(37, 0.9, np.float32)))
+    assert ids.tolist() == [osm.sample_row(x[0], v, top_p=np.float32(0.9))[0] for v in u]
+    assert torch.equal(ids, sample(ctx, t.repeat(37, 1), _cuda(u), top_p=_cuda(np.full(37, 0.9, np.float32))))
+    L = _lib.lib()
+    call = lambda stride, rows, vocab: L.vx_sample(ctx.h, t.data_ptr(), stride, rows, vocab, _cuda(u).data_ptr(), None, None,  # noqa: E731
+                                                   None, None, ids.data_ptr(), None, None)
+    assert [call(-1, 2, 100), call(0, -1, 100), call(0, 2 ** 20 + 1, 100), call(0, 1, 0), call(0, 1, 2 ** 18 + 1)] == [
+        _lib.VX_ERR_SHAPE] * 5

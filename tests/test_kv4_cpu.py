@@ -91,7 +91,7 @@ def test_cache_arguments_are_checked(host_cache):
         lambda: c.append(x, x, torch.zeros(2, dtype=torch.int32)), lambda: c.append(x, x, i, i.float()),
         lambda: c.append(torch.zeros(1, 3, 64, 2).transpose(2, 3), torch.zeros(1, 3, 64, 2).transpose(2, 3), i),
         lambda: c.append(x, torch.zeros(1, 6, 2, 64)[:, ::2], i), lambda: c.append(x[0], x[0], i),
-        lambda: c.read(1, i.long()), lambda: c.read(1, counts=torch.zeros(2, dtype=torch.int32)),
+        lambda: c.read(-1), lambda: c.read(1, i.long()), lambda: c.read(1, counts=torch.zeros(2, dtype=torch.int32)),
         lambda: c.attend(q.half(), i), lambda: c.attend(q[0], i), lambda: c.attend(torch.zeros(2, 256), i),
         lambda: c.attend(torch.zeros(1, 100), i), lambda: c.evict(i, i, 8, weights_out=torch.zeros(1, 2, 32)),
         lambda: c.evict(i, i, 8, positions_out=torch.zeros(1, 2, 64)),
@@ -104,6 +104,31 @@ def test_cache_arguments_are_checked(host_cache):
         with pytest.raises(VxError):
             call()
             raise AssertionError(f"call {n} was not refused")
+
+
+def test_strides_of_one_token_or_sequence_do_not_matter(host_cache, monkeypatch):
+    """A dimension of size 1 has no stride: rows that lie alike are not refused for it."""
+    import torch
+    got = []
+    lib = type("Lib", (), {"vx_kv4_append": lambda self, *a: got.append(a[4:7]) or 0})()
+    monkeypatch.setattr(host_cache, "_L", lib)
+    monkeypatch.setattr(host_cache, "_raw_stream", lambda i: 0)
+    i = torch.zeros(1, dtype=torch.int32)
+    dense, fused = torch.zeros(1, 1, 2, 64), torch.zeros(400).as_strided((1, 1, 2, 64), (390, 3, 64, 1))
+    assert dense.stride() != fused.stride()
+    host_cache.append(dense, fused, i)
+    host_cache.append(torch.zeros(1, 3, 2, 64), torch.zeros(5, 3, 2, 64)[2:3], i)
+    assert got == [(0, 0, 1), (0, 128, 3)]
+
+
+def test_plans_do_not_grow_without_end(host_cache, monkeypatch):
+    import torch
+    monkeypatch.setattr(host_cache, "_L", type("Lib", (), {"vx_kv4_attend_workspace": lambda self, *a: 0,
+                                                           "vx_kv4_attend": lambda self, *a: 0})())
+    monkeypatch.setattr(host_cache, "_raw_stream", lambda i: 0)
+    for n in range(3000):
+        host_cache.attend(torch.zeros(1, 256), torch.zeros(1, dtype=torch.int32), n)
+    assert len(host_cache._plans) <= 1024
 
 
 def test_sample_arguments_are_checked():

@@ -167,8 +167,9 @@ int kv4_check(vx_ctx* ctx, const vx_kv4* c, const char* what) {
     return fail(ctx, VX_ERR_SHAPE, "%s: head_dim must be 64 or 128 (got %d)", what, c->head_dim);
   if (c->batch <= 0 || c->n_kv_heads <= 0 || c->n_kv_heads > 32767 || (long long)c->batch * c->n_kv_heads > 65535)
     return fail(ctx, VX_ERR_SHAPE, "%s: batch * n_kv_heads must lie in 1..65535 (at most 32767 heads)", what);
-  if (c->capacity <= 0 || c->capacity % 32 != 0)
-    return fail(ctx, VX_ERR_SHAPE, "%s: capacity must be a positive multiple of 32 (got %d)", what, c->capacity);
+  if (c->capacity <= 0 || c->capacity % 32 != 0 || c->capacity > (1 << 30))
+    return fail(ctx, VX_ERR_SHAPE, "%s: capacity must be a positive multiple of 32 up to 2^30 (got %d)", what,
+                c->capacity);
   if (((uintptr_t)c->k_codes | (uintptr_t)c->k_scales | (uintptr_t)c->v_codes | (uintptr_t)c->v_scales) & 15)
     return fail(ctx, VX_ERR_ARG, "%s: cache buffers must be 16-byte aligned", what);
   return VX_OK;

@@ -354,7 +354,8 @@ extern "C" int vx_kv4_evict(vx_ctx* ctx, const vx_kv4* c, const int32_t* lens, c
   if (!lens || !seen || !lens_out || !weights_out || !positions_out)
     return fail(ctx, VX_ERR_ARG, "kv4_evict: lens, seen and the outputs are needed");
   if (!c->weights || !c->positions) return fail(ctx, VX_ERR_ARG, "kv4_evict: the cache keeps no weights and positions");
-  if (lens_out == lens) return fail(ctx, VX_ERR_ARG, "kv4_evict: lens_out must not be lens");
+  if (lens_out == lens || lens_out == seen)
+    return fail(ctx, VX_ERR_ARG, "kv4_evict: lens_out must be neither lens nor seen");
   if (max_len < 0 || max_len > c->capacity)
     return fail(ctx, VX_ERR_SHAPE, "kv4_evict: max_len %d outside 0..%d", max_len, c->capacity);
   if (max_len > EV_MAX_LEN) return fail(ctx, VX_ERR_SHAPE, "kv4_evict: max_len %d > %d", max_len, EV_MAX_LEN);

@@ -390,8 +390,9 @@ int ensure_batch(vx_lm* lm) {
   return VX_OK;
 }
 
-// Head for B rows (greedy, or sampling where lm->sampling is set): final norm (kept as the hidden the DiT consumes), logits over the
-// tied embedding, per-row pick -> token and next input embedding, then step (and position).
+// Head for B rows (greedy, or sampling where lm->sampling is set): final norm (kept as the hidden
+// the DiT consumes), logits over the tied embedding, per-row pick -> token and next input embedding,
+// then step (and position).
 int enqueue_batch_head(vx_lm* lm, int B, cudaStream_t st, bool advance_pos, bool normed = false) {
   vx_ctx* ctx = lm->ctx;
   const int H = lm->H;
@@ -1074,7 +1075,7 @@ int vx_lm_sample(vx_lm* lm, const int32_t* prompt_ids, int B, int n_prompt, int 
   if (B <= 0 || B > lm->max_batch || B > 128)
     return fail(ctx, VX_ERR_SHAPE, "batch %d outside 1..%d", B, std::min(lm->max_batch, 128));
   if (lm->V > (1 << 18)) return fail(ctx, VX_ERR_SHAPE, "sampling: vocabulary %d > 2^18", lm->V);
-  if (n_steps >= lm->max_length)
+  if (n_steps >= lm->max_length || n_prompt > lm->max_length)
     return fail(ctx, VX_ERR_KV_FULL, "KV cache is full: %d prompt + %d steps > %d", n_prompt, n_steps, lm->max_length);
   DeviceGuard guard(ctx->device);
   cudaStream_t st = ctx->stream;

@@ -890,7 +890,7 @@ extern "C" int vx_sample(vx_ctx* ctx, const float* logits, int64_t row_stride, i
   if (rows < 0 || rows > (1 << 20)) return fail(ctx, VX_ERR_SHAPE, "sample: %d rows outside 0..2^20", rows);
   if (vocab <= 0 || vocab > SP_MAX_VOCAB)
     return fail(ctx, VX_ERR_SHAPE, "sample: vocabulary %d outside 1..%d", vocab, SP_MAX_VOCAB);
-  if (row_stride < vocab) return fail(ctx, VX_ERR_SHAPE, "sample: row stride below the vocabulary");
+  if (row_stride < 0) return fail(ctx, VX_ERR_SHAPE, "sample: negative row stride");
   if (rows == 0) return VX_OK;
   DeviceGuard guard(ctx->device);
   VX_CUDA(ctx, launch_sample(logits, row_stride, rows, vocab, u, nullptr, temperature, top_k, top_p, min_p, ids, logprob,

@@ -31,7 +31,9 @@ class Kv4Cache:
     """A 4-bit cache of ``batch`` sequences: ``n_kv_heads`` heads of ``capacity`` rows (rounded up
     to a multiple of 32) of ``head_dim`` (64 or 128).  The filled lengths are the caller's: int32
     CUDA tensors of ``batch``, given to each call.  ``weights`` (the attention that each row has
-    received) and ``positions`` (int64) are kept with ``track=True``; ``evict`` needs them."""
+    received) and ``positions`` (int64) are kept with ``track=True``; ``evict`` needs them.  A length
+    outside its range leaves its sequence as it was (``attend``: NaN, ``read``: zeros), and the
+    context's next ``synchronize`` raises."""
 
     def __init__(self, ctx: Context, batch, n_kv_heads, capacity, head_dim, track=True):
         torch = _torch()
@@ -101,10 +103,13 @@ class Kv4Cache:
                 _refuse(VX_ERR_ARG, f"{what}: f32 on {self.device} is needed, got {t.dtype} on {t.device}")
         if s == 0:
             return
-        st = k.stride()
-        if st != v.stride() or st[3] != 1 or (st[2] != self.head_dim and self.n_kv_heads != 1):
+        st, sv, many = k.stride(), v.stride(), self.batch > 1
+        b_st, t_st = st[0] if many else 0, st[1] if s > 1 else 0  # of one alone the stride may be anything
+        alike = st == sv or (sv[3] == 1 and (sv[2] == st[2] or self.n_kv_heads == 1) and (sv[0] == b_st or not many)
+                             and (sv[1] == t_st or s == 1))
+        if not alike or st[3] != 1 or (st[2] != self.head_dim and self.n_kv_heads != 1):
             _refuse(VX_ERR_ARG, "k and v: dense heads and the same strides are needed")
-        rc = self._L.vx_kv4_append(self.ctx.h, self._ref, k.data_ptr(), v.data_ptr(), st[0], st[1], s,
+        rc = self._L.vx_kv4_append(self.ctx.h, self._ref, k.data_ptr(), v.data_ptr(), b_st, t_st, s,
                                    self._ints(start, "start"), self._ints(counts, "counts"),
                                    self._ints(first_position, "first_position"), self._raw_stream(self._index))
         if rc:
@@ -113,6 +118,8 @@ class Kv4Cache:
     def read(self, n, start=None, counts=None):
         """The values of rows ``start[b] + i`` (``i < counts[b] <= n``; zeros behind them) as
         ``k, v`` f32 ``[B, nkv, n, d]``."""
+        if n < 0:
+            _refuse(VX_ERR_SHAPE, f"read: {n} rows")
         k, v = self._empty((2, self.batch, self.n_kv_heads, n, self.head_dim), device=self.device).unbind(0)
         if n:
             rc = self._L.vx_kv4_read(self.ctx.h, self._ref, n, self._ints(start, "start"), self._ints(counts, "counts"),
@@ -136,6 +143,8 @@ class Kv4Cache:
         key = (width // d, n, bool(track))
         need = self._plans.get(key)
         if need is None:
+            if len(self._plans) >= 1024:  # a max_len that grows with every token
+                self._plans.clear()
             need = self._plans[key] = self._L.vx_kv4_attend_workspace(self._ref, *key)
         out = q.new_empty((batch, width))
         ws = self._empty(need, device=self.device, dtype=_torch().uint8) if need else None

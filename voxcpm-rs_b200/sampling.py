@@ -7,7 +7,8 @@ from .minicpm4 import Context, _torch, raw_stream
 
 
 def sample(ctx: Context, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, return_logprob=False):
-    """One id of each row of ``logits`` f32 ``[rows, vocab]`` (rows may be strided) drawn with the
+    """One id of each row of ``logits`` f32 ``[rows, vocab]`` (rows may be strided or
+    one row expanded) drawn with the
     random numbers ``u`` f32 ``[rows]`` in ``[0, 1)``.  ``temperature``, ``top_p``, ``min_p`` (f32)
     and ``top_k`` (int32) are CUDA tensors of ``rows``, or None for off; they apply in the order
     temperature, top-k, top-p, min-p.  Temperature 0 is the greedy pick.  Returns int32 ids (-1
