@@ -108,37 +108,37 @@ struct Row {
   const float* x;  // this block's logits
   int lo, cnt;     // their first index and number
   float lmax, floor_;
-  double lmax_d, inv_t;
+  double lmax_d, inv_t, per_16th;  // 1 / T; 16 / (T ln 2)
   const double* tab;
 
   __device__ __forceinline__ float at(int j) const { return IN_SHARED ? shared_row[j] : __ldg(x + j); }
 
-  // exp by a table of 2^(i/16) and a polynomial of degree 6 (table-driven, after Tang, 1989): off by
-  // less than 2^-50 of itself.  16 table entries of 8 bytes are all banks of shared memory once: a
-  // warp reads them without conflicts (a table of 64 with degree 4 took longer).  A token at
-  // z <= -31.5 has no weight (exp(-31.2) 2^44 = 1/2), nor has one next to +infinity or -infinity
-  // itself, where z is infinite or a NaN.
+  // exp(d / T) by a table of 2^(i/16) and a polynomial (table-driven, after Tang, 1989): with d / T in
+  // units of ln 2 / 16 split into an integer and x in [-1/2, 1/2], 2^(x/16) = 1 + x (c1 + .. + c5 x^4),
+  // Chebyshev's interpolation, off by less than 2^-46 of itself.  16 table entries of 8 bytes are all
+  // banks of shared memory once: a warp reads them without conflicts (a table of 64 with fewer terms
+  // took longer).  A token at z = d / T <= -31.5 has no weight (exp(-31.2) 2^44 = 1/2), nor has one
+  // next to +infinity or -infinity itself, where z is infinite or a NaN.
   // floor_: where lmax and the temperature are finite and ordinary, a logit at which z is below
   // -31.5, so that none from there down has a weight; else -infinity, and the cases are told apart.
   __device__ __forceinline__ u64 weight(float l) const {
-    if (floor_ > -INFINITY) return l > floor_ ? exp_of(((double)l - lmax_d) * inv_t) : 0;
-    const double z = l == lmax ? 0.0 : ((double)l - lmax_d) * inv_t;
-    return z > -31.5 ? exp_of(z) : 0;
+    if (floor_ > -INFINITY) return l > floor_ ? exp_of((double)l - lmax_d) : 0;
+    const double d = l == lmax ? 0.0 : (double)l - lmax_d;
+    return d * inv_t > -31.5 ? exp_of(d) : 0;
   }
-  __device__ __forceinline__ u64 exp_of(double z) const {
+  __device__ __forceinline__ u64 exp_of(double d) const {
     constexpr double kShift = 6755399441055744.0;  // 1.5 * 2^52: a sum with it is rounded to an integer
-    const double t = fma(z, 23.083120654223414215, kShift);         // 16 / ln 2
+    const double t = fma(d, per_16th, kShift);
     const int n = __double2loint(t);
-    const double r = fma(t - kShift, -0.043321698784996581839, z);  // ln 2 / 16; |r| <= 0.0217
-    double p = fma(r, 1.0 / 720, 1.0 / 120);
-    p = fma(p, r, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    p *= tab[n & 15];
-    const double s = __hiloint2double(__double2hiint(p) + ((n & ~15) << 16) + (SP_BITS << 20), __double2loint(p));
-    const double w = s + 4503599627370496.0;  // + 2^52: the nearest integer, in the low bits
+    const double x = fma(d, per_16th, kShift - t);
+    double p = fma(x, 1.2716049516906705e-09, 1.4676387238435006e-07);
+    p = fma(p, x, 1.3550807778387664e-05);
+    p = fma(p, x, 0.0009383847926296646);
+    p = fma(p, x, 0.04332169878499658);
+    p = fma(p, x, 1.0);
+    const double e = tab[n & 15];
+    const double s = __hiloint2double(__double2hiint(e) + ((n & ~15) << 16) + (SP_BITS << 20), __double2loint(e));
+    const double w = fma(p, s, 4503599627370496.0);  // + 2^52: the nearest integer, in the low bits
     return (u64)(__double2hiint(w) & 0xfffff) << 32 | (uint32_t)__double2loint(w);
   }
 };
@@ -210,7 +210,7 @@ __device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, cons
     } else if constexpr (KIND == SP_PLAIN) {
       u64 v[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) v[i] = row.exp_of(((double)fmaxf(l[i], row.floor_) - row.lmax_d) * row.inv_t);
+      for (int i = 0; i < U; ++i) v[i] = row.exp_of((double)fmaxf(l[i], row.floor_) - row.lmax_d);
 #pragma unroll
       for (int i = 0; i < U; ++i)
         if (l[i] > row.floor_) {
@@ -232,7 +232,7 @@ __device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, cons
   if constexpr (KIND == SP_MIDDLES) {
     __syncthreads();
     for (int i = exact + tid; i < Shared::kBuckets; i += Shared::kThreads) {
-      const u64 v = s.hist.lo[i] ? s.hist.lo[i] * row.exp_of(-(i + 0.5) / bucket.per * row.inv_t) : 0;
+      const u64 v = s.hist.lo[i] ? s.hist.lo[i] * row.exp_of(-(i + 0.5) / bucket.per) : 0;
       s.hist.lo[i] = (uint32_t)v;
       s.hist.hi[i] = (uint32_t)(v >> 32);
     }
@@ -396,7 +396,7 @@ __device__ Sums sum_all(Shared& s, const R& row, const Buckets<Shared>& bucket, 
     for (int i = 0; i < U; ++i) l[i] = j + 32 * i < j1 ? row.at(j + 32 * i) : -INFINITY;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      w[i] = row.exp_of(((double)fmaxf(l[i], row.floor_) - row.lmax_d) * row.inv_t);  // 0 at the floor
+      w[i] = row.exp_of((double)fmaxf(l[i], row.floor_) - row.lmax_d);  // 0 at the floor
       at[i] = (bucket.lmax - l[i]) * bucket.per;
     }
     bool some = false;
@@ -599,6 +599,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
     return;
   }
   row.inv_t = greedy ? 1.0 : 1.0 / (double)temp;
+  row.per_16th = row.inv_t * 23.083120654223414215;
   row.floor_ = -INFINITY;
   if (hi < INFINITY && row.inv_t > 1e-30 && row.inv_t < 1e30) {
     const float f = (float)(row.lmax_d - 32.0 / row.inv_t);
