@@ -189,23 +189,38 @@ __device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, cons
   for (int i = tid; i < Shared::kBuckets; i += Shared::kThreads) s.hist.lo[i] = s.hist.hi[i] = 0;
   __syncthreads();
   constexpr int U = 4;  // logits of a thread that are on their way together
-  // middles: the few tokens of weight above exp(-6) are added exactly, a large one's middle may be half
-  // a percent of all off
+  // middles: the few tokens of weight above exp(-6) are added by an f32 exponential, since a large one's
+  // middle may be half a percent of all off; to 28 places, of which each word of a sum takes 14, so that
+  // 2^18 of them fit and no carry is needed
   const int exact = KIND == SP_MIDDLES ? (int)fminf((float)(6.0 / row.inv_t) * bucket.per, (float)Shared::kBuckets) : 0;
+  const float per_two = KIND == SP_MIDDLES ? (float)(-1.4426950408889634 * row.inv_t) : 0.f;
+  constexpr bool AHEAD = KIND == SP_MIDDLES;  // read from L2: loads one round ahead
+  float next[U];
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) next[i] = j0 + i * Shared::kThreads < row.cnt ? row.at(j0 + i * Shared::kThreads) : -INFINITY;
+  };
+  if (AHEAD) load(tid);
   for (int j0 = tid; j0 < row.cnt; j0 += U * Shared::kThreads) {
+    if (!AHEAD) load(j0);
     float l[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) l[i] = j0 + i * Shared::kThreads < row.cnt ? row.at(j0 + i * Shared::kThreads) : -INFINITY;
+    for (int i = 0; i < U; ++i) l[i] = next[i];
+    if (AHEAD) load(j0 + U * Shared::kThreads);
     // plain rows: `per` is finite and no logit above the floor lies behind the last bucket
     if constexpr (KIND == SP_MIDDLES) {
 #pragma unroll
       for (int i = 0; i < U; ++i)
         if (l[i] > row.floor_) {
-          const int at = (int)((bucket.lmax - l[i]) * bucket.per);
-          if (at >= exact)
+          const float d = bucket.lmax - l[i];
+          const int at = (int)(d * bucket.per);
+          if (at >= exact) {
             atomicAdd(&s.hist.lo[at], 1u);
-          else
-            add64(&s.hist.lo[at], &s.hist.hi[at], row.weight(l[i]));
+          } else {
+            const uint32_t w = (uint32_t)exp2f(fmaf(d, per_two, 28.f));
+            atomicAdd(&s.hist.lo[at], w & 0x3fff);
+            atomicAdd(&s.hist.hi[at], w >> 14);
+          }
         }
     } else if constexpr (KIND == SP_PLAIN) {
       u64 v[U];
@@ -231,8 +246,12 @@ __device__ void find_bucket(cg::cluster_group& cl, Shared& s, const R& row, cons
   }
   if constexpr (KIND == SP_MIDDLES) {
     __syncthreads();
-    for (int i = exact + tid; i < Shared::kBuckets; i += Shared::kThreads) {
-      const u64 v = s.hist.lo[i] ? s.hist.lo[i] * row.exp_of(-(i + 0.5) / bucket.per) : 0;
+    for (int i = tid; i < Shared::kBuckets; i += Shared::kThreads) {
+      u64 v = 0;
+      if (i < exact)
+        v = (((u64)s.hist.hi[i] << 14) + s.hist.lo[i]) << (SP_BITS - 28);
+      else if (s.hist.lo[i])
+        v = s.hist.lo[i] * row.exp_of(-(i + 0.5) / bucket.per);
       s.hist.lo[i] = (uint32_t)v;
       s.hist.hi[i] = (uint32_t)(v >> 32);
     }
@@ -383,17 +402,24 @@ __device__ u64 sum_kept(Shared& s, const R& row, int j0, int j1, u64 least, Keep
 struct Sums {
   u64 all, sure, kept;
 };
-template <class Shared, class R>
+template <bool MIN_P, class Shared, class R>
 __device__ Sums sum_all(Shared& s, const R& row, const Buckets<Shared>& bucket, int j0, int j1, float from, float behind,
                         u64 least) {
   constexpr int U = 4;
   const int lane = threadIdx.x & 31;
   Sums t = {0, 0, 0};
+  float next[U];
+  auto load = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) next[i] = j + 32 * i < j1 ? row.at(j + 32 * i) : -INFINITY;
+  };
+  load(j0 + lane);
   for (int j = j0 + lane; j - lane < j1; j += U * 32) {
     float l[U], at[U];
     u64 w[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) l[i] = j + 32 * i < j1 ? row.at(j + 32 * i) : -INFINITY;
+    for (int i = 0; i < U; ++i) l[i] = next[i];
+    load(j + U * 32);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       w[i] = row.exp_of((double)fmaxf(l[i], row.floor_) - row.lmax_d);  // 0 at the floor
@@ -405,7 +431,7 @@ __device__ Sums sum_all(Shared& s, const R& row, const Buckets<Shared>& bucket, 
       t.all += w[i];
       if (at[i] < from) {
         t.sure += w[i];
-        if (w[i] >= least) t.kept += w[i];
+        if (MIN_P && w[i] >= least) t.kept += w[i];
       }
       some |= at[i] >= from && at[i] < behind;
     }
@@ -417,7 +443,7 @@ __device__ Sums sum_all(Shared& s, const R& row, const Buckets<Shared>& bucket, 
   }
   t.all = warp_sum64(t.all);
   t.sure = warp_sum64(t.sure);
-  t.kept = warp_sum64(t.kept);
+  t.kept = MIN_P ? warp_sum64(t.kept) : t.sure;
   return t;
 }
 
@@ -427,17 +453,18 @@ __device__ Sums sum_all(Shared& s, const R& row, const Buckets<Shared>& bucket, 
 template <class Shared>
 __device__ void sort_list(Shared& s, int n) {
   u64* ent = s.ent;
-  if (n <= Shared::kThreads / 4) {  // short: an entry's place is the number of larger ones, counted by four threads
+  if (n <= Shared::kThreads) {  // an entry's place is the number of larger ones, counted by 4, 2 or 1 threads
+    const int lg = n <= Shared::kThreads / 4 ? 2 : n <= Shared::kThreads / 2 ? 1 : 0;
     __syncthreads();  // the entries are there
-    const int i = threadIdx.x >> 2;
+    const int i = threadIdx.x >> lg, part = threadIdx.x & ((1 << lg) - 1);
     const u64 e = i < n ? ent[i] : 0;
     int larger = 0;
 #pragma unroll 4
-    for (int j = threadIdx.x & 3; j < n; j += 4) larger += ent[j] > e;
-    larger += __shfl_xor_sync(0xffffffffu, larger, 1);
-    larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+    for (int j = part; j < n; j += 1 << lg) larger += ent[j] > e;
+    if (lg > 0) larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+    if (lg > 1) larger += __shfl_xor_sync(0xffffffffu, larger, 2);
     __syncthreads();
-    if (i < n && (threadIdx.x & 3) == 0) ent[larger] = e;
+    if (i < n && part == 0) ent[larger] = e;
     __syncthreads();
     return;
   }
@@ -561,7 +588,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   // the row, its largest and its smallest finite logit, and whether it holds a NaN
   float hi = -INFINITY, lo = INFINITY;
   bool bad = false;
-#pragma unroll 8
+#pragma unroll (IN_SHARED ? 8 : 16)
   for (int j = tid; j < row.cnt; j += THREADS) {
     const float l = __ldg(row.x + j);
     if (IN_SHARED) shared_row[j] = l;
@@ -717,7 +744,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
       const float from = (float)max(0, s.bucket - (s.into < 0.25f)), behind = (float)(s.bucket + 1 + (s.into > 0.75f));
       if (tid == 0) s.n = 0;
       __syncthreads();
-      const Sums t = sum_all(s, row, bucket, w0, w1, from, behind, least);
+      const Sums t = least ? sum_all<true>(s, row, bucket, w0, w1, from, behind, least)
+                           : sum_all<false>(s, row, bucket, w0, w1, from, behind, least);
       if (lane == 0) {
         s.warp64[warp] = t.all;
         s.warp_sure[warp] = t.sure;
@@ -810,8 +838,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
   if (s.n >= 0) {  // one block of the cluster: all its warps walk the part of that warp
     u64 run = s.run;
     const int j0 = s.n * part, j1 = min(row.cnt, j0 + part);
+    float next = j0 + tid < j1 ? row.at(j0 + tid) : 0.f;
     for (int j = j0 + tid; j - tid < j1; j += THREADS) {
-      u64 w = j < j1 && stays(row.at(j), j) ? row.weight(row.at(j)) : 0;
+      const float l = next;
+      if (j + THREADS < j1) next = row.at(j + THREADS);
+      u64 w = j < j1 && stays(l, j) ? row.weight(l) : 0;
       if (w < least) w = 0;
       u64 incl = warp_scan64(w);
       __syncthreads();  // warp64 of the round before is read
