@@ -39,6 +39,7 @@ constexpr int SP_MAX_CLUSTER = 8;
 constexpr int SP_MAX_VOCAB = 1 << 18;  // sums of weights stay below 2^62
 constexpr int SP_THREADS = 512;
 constexpr int SP_BITS = 44;          // binary places of a weight
+constexpr int SP_MIDDLE_SLICE = 12288;  // tokens of a block from which a pass of exponentials costs more than a longer list
 constexpr double SP_ONE = (double)(1ull << SP_BITS);
 
 // 2^(i / 16)
@@ -736,10 +737,11 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(const SampleArgs 
       __syncthreads();
     };
     const bool plain = first == 0 && row.floor_ > -INFINITY && bucket.per > 0.f && bucket.per < 1e30f;
-    if (!IN_SHARED && plain) {
+    if (plain && a.slice >= SP_MIDDLE_SLICE) {
       // The bucket by middles, which may be off by one where the border lies near its end; then the
       // exact sums and a list of the bucket and that neighbour, each token's weight computed once (256
-      // rows of 151643 tokens 288 -> 240 us; with few rows the longer list costs more than that saves).
+      // rows of 151643 tokens 288 -> 240 us, 64 rows of 73448 41 -> 37; slices of 9181 tokens gain
+      // nothing, 8 rows of 73448 with mixed settings 23.5 -> 24.3).
       find_bucket<SP_MIDDLES>(cl, s, row, bucket, [](float, int) { return (u64)0; }, need_of);
       const float from = (float)max(0, s.bucket - (s.into < 0.25f)), behind = (float)(s.bucket + 1 + (s.into > 0.75f));
       if (tid == 0) s.n = 0;
