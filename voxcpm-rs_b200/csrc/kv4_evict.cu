@@ -307,12 +307,17 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
   cl.sync();  // the lists are read by the other blocks
 }
 
-// Blocks of a cluster and keys of a thread: as many blocks as keep about two on each SM (one, where
-// that takes clusters above 8, of which fewer fit a GPC: 16 units of 32768 rows 21 us at 8 and 36 at
-// 16, but 8 units of 125000 rows 83 and 59), as few keys as hold the longest sequence.
+// Blocks of a cluster and keys of a thread.  More blocks scan faster, but clusters of 8 and more cost
+// more to launch and to bring together, the more so where several share a GPC.  So they double while a
+// thread would have more than 4 keys (from 4 to 8 blocks: 5) and the blocks are few: two to an SM, for
+// 16 in a cluster one (16 units of 4160 rows: 4 blocks 10.4 us, 8 14.1; of 16000: 4 29.0, 8 25.0, 16
+// 43.0; 32 units of 32749: 4 36.2, 8 28.6, 16 62.2; 64 units of 16000: 2 46.2, 4 34.9, 8 45.7).  The
+// keys of a thread are as few as hold the longest sequence.
 void evict_shape(int units, int max_len, int* C, int* items) {
   *C = 1;
-  while (*C < EV_MAX_CLUSTER && max_len > EV_THREADS * 2 * *C && units * *C * 2 <= (*C < 8 ? 296 : 148)) *C *= 2;
+  while (*C < EV_MAX_CLUSTER && max_len > EV_THREADS * (*C == 4 ? 5 : 4) * *C &&
+         (long long)units * *C * 2 <= (*C < 8 ? 296 : 148))
+    *C *= 2;
   while (max_len > EV_THREADS * EV_MAX_ITEMS * *C) *C *= 2;
   *items = 2;
   while (max_len > EV_THREADS * *items * *C) *items *= 2;
