@@ -115,16 +115,21 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
   }
   const int base = (rank * EV_WARPS + warp) * 32 * ITEMS + lane;  // slot of item i: base + 32 i
   const int64_t since = (int64_t)a.seen[b] - a.recent;
+  constexpr int G = ITEMS < 8 ? ITEMS : 8;  // rows of a thread that are on their way together
   uint32_t key[ITEMS];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int j = base + 32 * i;
-    key[i] = 0;
-    if (j < n) {
-      const int64_t pos = a.positions[row0 + j];
-      const float w = a.weights[row0 + j];
-      key[i] = (pos < a.sink || pos >= since) ? 0xffffffffu : weight_key(w);
+  for (int i0 = 0; i0 < ITEMS; i0 += G) {
+    float w[G];
+    int64_t pos[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int j = min(base + 32 * (i0 + i), n - 1);
+      w[i] = a.weights[row0 + j];
+      pos[i] = a.positions[row0 + j];
     }
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      key[i0 + i] = base + 32 * (i0 + i) >= n ? 0 : pos[i] < a.sink || pos[i] >= since ? 0xffffffffu : weight_key(w[i]);
   }
   if (tid < 256) s.hist[0][tid] = 0;
   __syncthreads();
@@ -234,7 +239,6 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
   // rows that stay where they are: loads of eight at a time, ahead of the stores that may alias them
   const bool apart = a.weights_out != a.weights || a.positions_out != a.positions;
   if (apart && (rank * EV_WARPS + warp) * 32 * ITEMS < a.keep) {
-    constexpr int G = ITEMS < 8 ? ITEMS : 8;
 #pragma unroll
     for (int i0 = 0; i0 < ITEMS; i0 += G) {
       float w[G];
