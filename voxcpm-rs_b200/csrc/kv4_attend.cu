@@ -73,6 +73,7 @@ __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
 constexpr int AT_WARPS = 4;
 constexpr int AT_TILE = 32;   // positions of a tile
 constexpr int AT_STAGES = 3;  // tiles of a warp in shared memory
+constexpr int AT_MAX_CLUSTER = 8;  // splits that a cluster joins
 
 // The dim of column c of a split's sums: columns are ordered by m-tile, then g, then the pair.
 template <int D>
@@ -441,11 +442,15 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 4 : 5) kv4_split_ker
     float* fin = joined + HB * 2;  // [8][2]: maximum and 1 / sum over the cluster
     if (tid < heads) {  // where the weights or other blocks' sums need it
       float M = -INFINITY, L = 0.f;
-      for (int r = 0; r < C; ++r) M = fmaxf(M, cl.map_shared_rank(joined, r)[tid * 2]);
-      for (int r = 0; r < C; ++r) {
-        const float* p = cl.map_shared_rank(joined, r) + tid * 2;
-        L = fmaf(ex2(p[0] - M), p[1], L);
-      }
+      float2 ml[AT_MAX_CLUSTER];  // unconditional loads: one round trip for all blocks
+#pragma unroll
+      for (int r = 0; r < AT_MAX_CLUSTER; ++r)
+        ml[r] = *reinterpret_cast<const float2*>(cl.map_shared_rank(joined, min(r, C - 1)) + tid * 2);
+#pragma unroll
+      for (int r = 0; r < AT_MAX_CLUSTER; ++r) M = fmaxf(M, ml[r].x);
+#pragma unroll
+      for (int r = 0; r < AT_MAX_CLUSTER; ++r)
+        if (r < C) L = fmaf(ex2(ml[r].x - M), ml[r].y, L);
       fin[tid * 2] = M;
       fin[tid * 2 + 1] = 1.f / L;
     }
@@ -632,7 +637,6 @@ __global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, in
   }
 }
 
-constexpr int AT_MAX_CLUSTER = 8;    // splits that a cluster joins
 constexpr int AT_CLUSTER_CHUNK = 512;  // their positions at most: the scores of a tracking call lie in shared memory
 
 struct AttendPlan {

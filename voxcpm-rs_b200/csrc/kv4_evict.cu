@@ -145,13 +145,23 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
     }
     cl.sync();
     if (tid < 256) {
-      uint32_t t = 0;
+      // unconditional loads, all on their way together: one round trip for four or eight blocks
+      uint32_t t = 0, v[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r)  // unrolled: one round trip for eight blocks
-        if (r < C) t += cl.map_shared_rank(h, r)[tid];
+      for (int r = 0; r < 4; ++r) v[r] = cl.map_shared_rank(h, min(r, C - 1))[tid];
+      if (C > 4) {
+#pragma unroll
+        for (int r = 4; r < 8; ++r) v[r] = cl.map_shared_rank(h, r)[tid];
+#pragma unroll
+        for (int r = 4; r < 8; ++r) t += v[r];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t += r < C ? v[r] : 0;
       if (C > 8) {
 #pragma unroll
-        for (int r = 8; r < 16; ++r) t += cl.map_shared_rank(h, r)[tid];
+        for (int r = 0; r < 8; ++r) v[r] = cl.map_shared_rank(h, r + 8)[tid];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) t += v[r];
       }
       s.tot[tid] = t;
     }
