@@ -492,10 +492,17 @@ __device__ __forceinline__ void head_stats(const AttendArgs& a, int unit, int r,
   const int lane = threadIdx.x & 31;
   const float2* p = reinterpret_cast<const float2*>(a.part_ml) + (size_t)unit * a.nsplit * HB + r;
   float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < active; s += 32) {  // each lane's own running maximum, joined below
-    const float2 x = p[(size_t)s * HB];
-    const float mn = fmaxf(m, x.x);
-    l = l * ex2(m - mn) + x.y * ex2(x.x - mn);
+  constexpr int U = 8;
+  for (int s = lane; s < active; s += 32 * U) {  // each lane's own running maximum, joined below
+    float2 x[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) x[i] = s + 32 * i < active ? p[(size_t)(s + 32 * i) * HB] : make_float2(-INFINITY, 0.f);
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < U; ++i) mn = fmaxf(mn, x[i].x);
+    l *= ex2(m - mn);
+#pragma unroll
+    for (int i = 0; i < U; ++i) l = fmaf(x[i].y, ex2(x[i].x - mn), l);
     m = mn;
   }
   *M = warp_max(m);
@@ -516,6 +523,7 @@ __device__ __forceinline__ void merge_few(const AttendArgs& a, int unit) {
   const int h = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hb = unit % a.nhb, g = (unit / a.nhb) % a.nkv, b = unit / (a.nhb * a.nkv);
   const int n = seq_len(a, b);
+  pdl_wait();
   if (n <= 0 || h >= HB || hb * HB + h >= a.nrep) return;
   const int active = (n + a.chunk - 1) / a.chunk;
   float2 ml = make_float2(-INFINITY, 0.f);
@@ -547,7 +555,7 @@ __global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, in
                                                           int chunks) {
   extern __shared__ __align__(16) float4 acc[];  // one for each thread
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_wait();
+  // lengths and weights are not the split kernel's: they are read before it has ended
   if ((int)blockIdx.x < merge_blocks && a.nsplit <= FIN_FEW) {
     merge_few<D>(a, blockIdx.x);
     return;
@@ -556,22 +564,38 @@ __global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, in
     const int slice = blockIdx.x % slices, r = blockIdx.x / slices % HB, unit = blockIdx.x / (slices * HB);
     const int hb = unit % a.nhb, g = (unit / a.nhb) % a.nkv, b = unit / (a.nhb * a.nkv);
     const int n = seq_len(a, b);
+    pdl_wait();
     if (n <= 0 || hb * HB + r >= a.nrep) return;
     const int active = (n + a.chunk - 1) / a.chunk;
     const int lps = D / 4 / slices, groups = blockDim.x / lps, grp = tid / lps, l4 = slice * lps + tid % lps;
-    float M, inv;
-    head_stats(a, unit, r, active, &M, &inv);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     const float* ml = a.part_ml + ((size_t)unit * a.nsplit * HB + r) * 2;
     const float4* po = reinterpret_cast<const float4*>(a.part_o + ((size_t)unit * a.nsplit * HB + r) * D) + l4;
-#pragma unroll 4
-    for (int s = grp; s < active; s += groups) {
-      const float f = ex2(ml[(size_t)s * HB * 2] - M);
-      const float4 x = po[(size_t)s * HB * (D / 4)];
-      o.x = fmaf(f, x.x, o.x);
-      o.y = fmaf(f, x.y, o.y);
-      o.z = fmaf(f, x.z, o.z);
-      o.w = fmaf(f, x.w, o.w);
+    constexpr int U = 4;  // splits of a thread on their way together, the first before the statistics are there
+    float f[U];
+    float4 x[U];
+    auto load = [&](int s0) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int s = min(s0 + i * groups, active - 1);
+        f[i] = s0 + i * groups < active ? ml[(size_t)s * HB * 2] : -INFINITY;
+        x[i] = po[(size_t)s * HB * (D / 4)];
+      }
+    };
+    load(grp);
+    float M, inv;
+    head_stats(a, unit, r, active, &M, &inv);
+    for (int s = grp; s < active; s += U * groups) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (s + i * groups >= active) break;
+        const float e = ex2(f[i] - M);
+        o.x = fmaf(e, x[i].x, o.x);
+        o.y = fmaf(e, x[i].y, o.y);
+        o.z = fmaf(e, x[i].z, o.z);
+        o.w = fmaf(e, x[i].w, o.w);
+      }
+      if (s + U * groups < active) load(s + U * groups);
     }
     acc[tid] = o;
     for (int half = groups / 2; half > 0; half /= 2) {  // the groups, two by two
@@ -593,7 +617,10 @@ __global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, in
   const int i = blockIdx.x - merge_blocks;
   const int c = i % chunks, bg = i / chunks, b = bg / a.nkv;
   const int n = seq_len(a, b), j0 = c * FIN_POS * (int)blockDim.x + tid;
-  if (n <= 0 || j0 - tid >= n) return;
+  if (n <= 0 || j0 - tid >= n) {
+    pdl_wait();
+    return;
+  }
   const int active = (n + a.chunk - 1) / a.chunk;
   float w[FIN_POS], got[FIN_POS];
 #pragma unroll
@@ -602,6 +629,7 @@ __global__ void __launch_bounds__(1024) kv4_finish_kernel(const AttendArgs a, in
     w[u] = j < n ? a.weights[(size_t)bg * a.cap + j] : 0.f;
     got[u] = 0.f;
   }
+  pdl_wait();
   for (int hb = 0; hb < a.nhb; ++hb) {
     const int unit = bg * a.nhb + hb, heads = min(HB, a.nrep - hb * HB);
     float4 s[FIN_POS][2];
