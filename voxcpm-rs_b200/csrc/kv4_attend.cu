@@ -72,7 +72,10 @@ __device__ __forceinline__ int seq_len(const AttendArgs& a, int b) {
 //     it both kinds of shared-memory reads are free of bank conflicts.
 constexpr int AT_WARPS = 4;
 constexpr int AT_TILE = 32;   // positions of a tile
-constexpr int AT_STAGES = 3;  // tiles of a warp in shared memory
+// Tiles of a warp in shared memory.  2 where the scores of a tracking call lie beside them and all its
+// blocks are on the GPU at once if four fit on an SM, not three (64 units of 4000 rows in 512 blocks: 3
+// tiles 29.8 us, 2 21.8; 2 units in 16 blocks: 11.0 and 11.7; 200 ragged units in 800: 31.3 and 34.1).
+constexpr int AT_STAGES = 3, AT_FEW_STAGES = 2;
 constexpr int AT_MAX_CLUSTER = 8;  // splits that a cluster joins
 
 // The dim of column c of a split's sums: columns are ordered by m-tile, then g, then the pair.
@@ -164,7 +167,7 @@ struct TileLoader {
   }
 };
 
-template <int D, bool CLUSTER>
+template <int D, bool CLUSTER, int STAGES>
 __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 4 : 5) kv4_split_kernel(const AttendArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int KS = D / 16;  // k-steps of S, m-tiles of O^T
@@ -192,14 +195,14 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 4 : 5) kv4_split_ker
   const int j0 = split * a.chunk, j1 = min(n, j0 + a.chunk);
   if (!CLUSTER && j0 >= j1) return;
   const size_t row0 = (size_t)(b * a.nkv + g0) * a.cap;
-  float* own_scores = reinterpret_cast<float*>(smem + AT_WARPS * AT_STAGES * TileBytes<D>::all);  // [chunk][8]
-  uint8_t* ring = smem + warp * (AT_STAGES * TileBytes<D>::all);
+  float* own_scores = reinterpret_cast<float*>(smem + AT_WARPS * STAGES * TileBytes<D>::all);  // [chunk][8]
+  uint8_t* ring = smem + warp * (STAGES * TileBytes<D>::all);
   const int first = j0 + warp * AT_TILE;
   const int tiles = first < j1 ? (j1 - first + AT_WARPS * AT_TILE - 1) / (AT_WARPS * AT_TILE) : 0;
   TileLoader<D> loader;
   loader.init(a, row0 + first, ring, lane);
 #pragma unroll
-  for (int i = 0; i < AT_STAGES - 1; ++i) {
+  for (int i = 0; i < STAGES - 1; ++i) {
     if (i < tiles) loader.load(i, j1 - (first + i * AT_WARPS * AT_TILE));
     cp_async_commit();
   }
@@ -244,10 +247,10 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 4 : 5) kv4_split_ker
   const int vs_off[2] = {v_scales + t * (D / 16) + v_group, v_scales + (7 - t) * (D / 16) + v_group};
 
   for (int it = 0; it < tiles; ++it) {
-    cp_async_wait<AT_STAGES - 2>();
+    cp_async_wait<STAGES - 2>();
     __syncwarp();
     const int p0 = first + it * AT_WARPS * AT_TILE;
-    const uint8_t* st = ring + (it % AT_STAGES) * TileBytes<D>::all;
+    const uint8_t* st = ring + (it % STAGES) * TileBytes<D>::all;
     float s[8];  // n-tile i's columns 2t, 2t + 1 at 2i, 2i + 1
 #pragma unroll
     for (int i2 = 0; i2 < 2; ++i2) {  // two n-tiles at a time
@@ -375,8 +378,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, D == 128 ? 4 : 5) kv4_split_ker
         for (int e = 0; e < 4; ++e) o[4 * q + j][e] += c[j][e];
     }
     __syncwarp();  // every lane has read the stage that the next load goes into
-    const int nx = it + AT_STAGES - 1;
-    if (nx < tiles) loader.load(nx % AT_STAGES, j1 - (first + nx * AT_WARPS * AT_TILE));
+    const int nx = it + STAGES - 1;
+    if (nx < tiles) loader.load(nx % STAGES, j1 - (first + nx * AT_WARPS * AT_TILE));
     cp_async_commit();
   }
   cp_async_wait<0>();
@@ -712,23 +715,26 @@ AttendPlan plan_of(const vx_kv4* c, int nh, int max_len, int track) {
   return p;
 }
 
-constexpr size_t split_smem(int d) {
-  return AT_WARPS * AT_STAGES * (d == 128 ? TileBytes<128>::all : TileBytes<64>::all);
+constexpr size_t split_smem(int d, int stages) {
+  return AT_WARPS * stages * (d == 128 ? TileBytes<128>::all : TileBytes<64>::all);
 }
-constexpr size_t cluster_smem(int d, int chunk, bool track) {
-  return split_smem(d) + (track ? (size_t)chunk * HB * 4 : 0);
+constexpr size_t cluster_smem(int d, int stages, int chunk, bool track) {
+  return split_smem(d, stages) + (track ? (size_t)chunk * HB * 4 : 0);
 }
 
 template <int D>
 cudaError_t launch_split(const AttendArgs& a, const AttendPlan& p, int units, cudaStream_t st) {
   if (!p.cluster) {
-    kv4_split_kernel<D, false><<<dim3(p.nsplit, units), AT_WARPS * 32, split_smem(D), st>>>(a);
+    kv4_split_kernel<D, false, AT_STAGES>
+        <<<dim3(p.nsplit, units), AT_WARPS * 32, split_smem(D, AT_STAGES), st>>>(a);
     return cudaGetLastError();
   }
+  const int blocks = units * p.nsplit;
+  const bool track = a.weights != nullptr, few = D == 128 && track && blocks > 148 * 3 && blocks <= 148 * 4;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.nsplit, units);
   cfg.blockDim = dim3(AT_WARPS * 32);
-  cfg.dynamicSmemBytes = cluster_smem(D, p.chunk, a.weights != nullptr);
+  cfg.dynamicSmemBytes = cluster_smem(D, few ? AT_FEW_STAGES : AT_STAGES, p.chunk, track);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -737,16 +743,22 @@ cudaError_t launch_split(const AttendArgs& a, const AttendPlan& p, int units, cu
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.nsplit > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kv4_split_kernel<D, true>, a);
+  if constexpr (D == 128)
+    if (few) return cudaLaunchKernelEx(&cfg, kv4_split_kernel<D, true, AT_FEW_STAGES>, a);
+  return cudaLaunchKernelEx(&cfg, kv4_split_kernel<D, true, AT_STAGES>, a);
 }
 
 template <int D>
 cudaError_t configure_split() {
-  const cudaError_t e = cudaFuncSetAttribute(kv4_split_kernel<D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)split_smem(D));
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(kv4_split_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)cluster_smem(D, AT_CLUSTER_CHUNK, true));
+  const int most = (int)cluster_smem(D, AT_STAGES, AT_CLUSTER_CHUNK, true);
+  auto allow = [&](void (*kernel)(AttendArgs)) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  };
+  cudaError_t e = allow(kv4_split_kernel<D, false, AT_STAGES>);
+  if (e == cudaSuccess) e = allow(kv4_split_kernel<D, true, AT_STAGES>);
+  if constexpr (D == 128)
+    if (e == cudaSuccess) e = allow(kv4_split_kernel<D, true, AT_FEW_STAGES>);
+  return e;
 }
 
 }  // namespace
