@@ -15,7 +15,7 @@
 // the issue slots and, measured with nothing else around them, take 103 clocks together.  Long
 // batches run at 3.9 TB/s (64 sequences of 32768 rows: 153 us; floor 94); short ones are bound by
 // latency: launch, first tile, merge (one sequence of 64 rows 4.5 us, of 1001 rows in a cluster of
-// 8 splits 5.9 us).
+// 8 splits 5.3 us).
 #include <cooperative_groups.h>
 
 #include <cfloat>

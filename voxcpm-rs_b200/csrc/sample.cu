@@ -15,12 +15,13 @@
 // The draw takes the first token in index order whose running sum of staying weights exceeds
 // u * total: sums of each warp's part of the row, then one block walks the part that holds it.
 //
-// What bounds it: with many rows of which every token needs its weight, instruction issue in the pass
-// that computes it (13 f64 operations and a table read for each token) and the shared-memory atomics of
-// the counting pass before (256 rows of 151643 tokens 240 us, where reading them takes 24); with few
-// rows the round trips between the blocks (each about half a microsecond; six of them; one row of
-// 73448 tokens 16 us).  A 64-bit sum takes two 32-bit atomics, 3.7 clocks of an SM for 32 tokens, where
-// one 64-bit atomic is a compare-and-swap loop of 30.
+// What bounds it: with many rows of which every token needs its weight, instruction issue and latency in
+// the pass that computes it (11 f64 operations and a table read for each token), the shared-memory
+// atomics of the counting pass before, and the read, which take about 60, 50 and 37 thousand clocks of
+// a block (256 rows of 151643 tokens 183 us, where reading them alone takes 24); with few rows the round
+// trips between the blocks (each about half a microsecond; six of them; one row of 73448 tokens 14 us).
+// A 64-bit sum takes two 32-bit atomics, 3.7 clocks of an SM for 32 tokens, where one 64-bit atomic is
+// a compare-and-swap loop of 30.
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -39,7 +40,7 @@ constexpr int SP_MAX_CLUSTER = 8;
 constexpr int SP_MAX_VOCAB = 1 << 18;  // sums of weights stay below 2^62
 constexpr int SP_THREADS = 512;
 constexpr int SP_BITS = 44;          // binary places of a weight
-constexpr int SP_MIDDLE_SLICE = 12288;  // tokens of a block from which a pass of exponentials costs more than a longer list
+constexpr int SP_MIDDLE_SLICE = 12288;  // tokens of a block for which another exponential each costs more than a longer list
 constexpr double SP_ONE = (double)(1ull << SP_BITS);
 
 // 2^(i / 16)
@@ -882,8 +883,8 @@ struct SampleShape {
 constexpr int SP_SLICE = 32768;  // logits of a block in shared memory at most: 128 KB
 constexpr int SP_TWO = 18432;    // that leave room for two blocks on an SM
 // As many blocks of a row as there are SMs for (one row of 73448 tokens: 8 blocks 15 us, 2 blocks
-// 27 us; 64 rows: 4 blocks 38 us, 8 blocks 52 us).  256 rows of 151643 tokens: 2 blocks that read L2
-// 240 us (288 without the middles), 8 with the row in shared memory 347 us.
+// 27 us; 64 rows: 4 blocks 43 us, 8 blocks 57 us).  256 rows of 151643 tokens that are read from L2: 1
+// block 252 us, 2 232, 4 249, 8 381; 8 with the row in shared memory 345 us (2 blocks by now: 183).
 SampleShape shape_of(int rows, int vocab) {
   SampleShape p = {1, true};
   while (p.blocks < SP_MAX_CLUSTER && vocab > 2048 * p.blocks && rows * p.blocks < 148) p.blocks *= 2;
