@@ -111,13 +111,14 @@ def test_sample_follows_the_distribution(ctx):
     assert np.all(np.diff(ids) >= 0)
 
 
-@pytest.mark.parametrize("kw", [{}, dict(k=1), dict(k=700), dict(k=15000), dict(p=0.3), dict(p=0.97), dict(p=0.9, mp=0.1),
-                                dict(k=2000, p=0.5), dict(T=0.05, p=0.8), dict(T=30.0, p=0.5), dict(T=1e35, p=0.5)])
-def test_sample_many_rows(ctx, kw):
-    """The form for many rows (read from L2): rows where the list is too short, the border lies at a
-    bucket's end, or nothing is ordinary.  20 copies of 8 rows give the same ids."""
+@pytest.mark.parametrize("kw", [{}, dict(k=1), dict(k=700), dict(k=15000), dict(p=0.2), dict(p=0.3), dict(p=0.97),
+                                dict(p=0.9, mp=0.1), dict(k=2000, p=0.5), dict(T=0.05, p=0.8), dict(T=30.0, p=0.5), dict(T=1e35, p=0.5)])
+@pytest.mark.parametrize("V", [15011, 20011, 30011])
+def test_sample_many_rows(ctx, V, kw):
+    """The forms for many rows (in shared memory or read from L2, with and without the counting pass):
+    rows where the list is too short, the border lies at a bucket's end or far from where the count puts
+    it, or nothing is ordinary.  20 copies of 9 rows give the same ids."""
     rng = np.random.default_rng(11)
-    V = 20011
     base = (rng.standard_normal(V) * 2.5).astype(np.float32)
     peaks = base.copy()
     peaks[rng.integers(0, V, 6)] += 14
@@ -125,17 +126,21 @@ def test_sample_many_rows(ctx, kw):
     lowest = np.where(rng.random(V) < 0.5, np.finfo(np.float32).min, base).astype(np.float32)
     two = rng.integers(0, 2, V).astype(np.float32)
     pinf = base.copy()
-    pinf[[3, 19999]] = np.inf
+    pinf[[3, V - 12]] = np.inf
     near = (np.round(base * 4) / 4).astype(np.float32)
-    rows = np.stack([base, peaks, masked, lowest, two, pinf, near, np.zeros(V, np.float32)])
+    # most of the weight at one logit, half a bucket from its bucket's middle, behind a few that hold the border
+    off = np.full(V, -40.0, np.float32)
+    off[1:2001], off[2001:12001], off[0] = rng.uniform(-6.9, -6.1, 2000), -7.0, 0.0
+    off = off[rng.permutation(V)]
+    rows = np.stack([base, peaks, masked, lowest, two, pinf, near, np.zeros(V, np.float32), off])
     from voxcpm_rs_b200.sampling import sample
     args = {n: kw.get(s) for n, s in (("temperature", "T"), ("top_k", "k"), ("top_p", "p"), ("min_p", "mp"))}
-    full = {n: None if v is None else _cuda(np.full(160, v, np.int32 if n == "top_k" else np.float32)) for n, v in args.items()}
+    full = {n: None if v is None else _cuda(np.full(180, v, np.int32 if n == "top_k" else np.float32)) for n, v in args.items()}
     for u in (0.0, 0.4321, 0.99):
         want = [osm.sample_row(r, np.float32(u), np.float32(kw.get("T", 1.0)), kw.get("k", 0), np.float32(kw.get("p", 1.0)),
                                np.float32(kw.get("mp", 0.0)))[0] for r in rows]
-        ids = sample(ctx, _cuda(np.tile(rows, (20, 1))), _cuda(np.full(160, u, np.float32)), **full).cpu().numpy()
-        assert ids.reshape(20, 8).tolist() == [want] * 20, u
+        ids = sample(ctx, _cuda(np.tile(rows, (20, 1))), _cuda(np.full(180, u, np.float32)), **full).cpu().numpy()
+        assert ids.reshape(20, 9).tolist() == [want] * 20, u
 
 
 def test_sample_one_row_for_many_draws(ctx):
