@@ -201,6 +201,16 @@ def test_attend_ragged(ctx, d, lens, max_len, cap):
     _check_attend(ctx, np.random.default_rng(len(lens)), len(lens), 2, 8, d, max_len, lens, True, cap)
 
 
+@pytest.mark.parametrize("B,max_len", [(32, 1000), (60, 1400), (37, 515)])
+@pytest.mark.parametrize("track", [False, True])
+def test_attend_many_sequences(ctx, B, max_len, track):
+    """Blocks of all sequences on the GPU at once: fewer tiles in flight where they track."""
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, max_len + 1, B)
+    lens[:3] = max_len, 0, 1
+    _check_attend(ctx, rng, B, 2, 8, 128, max_len, lens, track)
+
+
 def test_attend_large_scores(ctx):
     """Scores of hundreds, the largest at the end: the running maximum grows in every tile, and
     rows far below it vanish."""
@@ -299,6 +309,14 @@ def test_evict(ctx, d, n, keep, sink, recent, inplace):
 def test_evict_ragged(ctx):
     """Sequences at, below and above the budget, an empty one among them, in one call."""
     _check_evict(ctx, np.random.default_rng(1), 6, 2, 128, 9000, [0, 1, 600, 601, 8999, 4000], 600, 4, 100, max_len=8999)
+
+
+@pytest.mark.parametrize("B,n", [(1, 1025), (1, 2049), (1, 4097), (1, 10241), (1, 16385), (36, 4100), (40, 2500), (75, 2049)])
+def test_evict_shapes(ctx, B, n):
+    """Either side of where more blocks share a sequence, for few sequences and for many."""
+    rng = np.random.default_rng(n)
+    lens = np.concatenate([[n], rng.integers(0, n + 1, B - 1)])
+    _check_evict(ctx, rng, B, 2, 64, -(-n // 32) * 32, lens, n // 2 + 1, 4, 100)
 
 
 def test_evict_long(ctx):
