@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 struct EvictShared {
-  uint32_t hist[3][256], tot[256];
+  alignas(16) uint32_t hist[3][256], tot[256];
   uint32_t warp_n[2][EV_WARPS];
   uint32_t eq, holes, movers;  // of this block; read by the cluster
 };
@@ -87,7 +87,7 @@ __device__ __forceinline__ void move_pieces(uint32_t n, int tid, Where where) {
 }
 
 template <int ITEMS>
-__global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(EV_THREADS, 2) kv4_evict_kernel(const EvictArgs a) {
   extern __shared__ __align__(16) uint32_t list[];  // free slots from the front, movers from the back
   uint32_t* to = list + EV_THREADS * ITEMS;         // the slots that this block's movers take
   __shared__ EvictShared s;
@@ -144,26 +144,30 @@ __global__ void __launch_bounds__(EV_THREADS) kv4_evict_kernel(const EvictArgs a
         atomicAdd(&h[(key[i] >> shift) & 255], 1u);
     }
     cl.sync();
-    if (tid < 256) {
-      // unconditional loads, all on their way together: one round trip for four or eight blocks
-      uint32_t t = 0, v[8];
+    if (tid < 128) {
+      // unconditional loads of two counts, all on their way together: a round trip for four or eight
+      // blocks (loads of one count: 32 units of 32749 rows 23.1 instead of 21.9 us)
+      uint2 t = make_uint2(0, 0), v[8];
+      auto at = [&](int r) { return reinterpret_cast<const uint2*>(cl.map_shared_rank(h, r))[tid]; };
+      auto add = [&](const uint2& x) { t.x += x.x, t.y += x.y; };
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = cl.map_shared_rank(h, min(r, C - 1))[tid];
+      for (int r = 0; r < 4; ++r) v[r] = at(min(r, C - 1));
       if (C > 4) {
 #pragma unroll
-        for (int r = 4; r < 8; ++r) v[r] = cl.map_shared_rank(h, r)[tid];
+        for (int r = 4; r < 8; ++r) v[r] = at(r);
 #pragma unroll
-        for (int r = 4; r < 8; ++r) t += v[r];
+        for (int r = 4; r < 8; ++r) add(v[r]);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t += r < C ? v[r] : 0;
+      for (int r = 0; r < 4; ++r)
+        if (r < C) add(v[r]);
       if (C > 8) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = cl.map_shared_rank(h, r + 8)[tid];
+        for (int r = 0; r < 8; ++r) v[r] = at(r + 8);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) t += v[r];
+        for (int r = 0; r < 8; ++r) add(v[r]);
       }
-      s.tot[tid] = t;
+      reinterpret_cast<uint2*>(s.tot)[tid] = t;
     }
     __syncthreads();
     // every warp finds the digit at which the count from above reaches `left`
