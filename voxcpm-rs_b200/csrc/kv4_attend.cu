@@ -701,14 +701,26 @@ AttendPlan plan_of(const vx_kv4* c, int nh, int max_len, int track) {
     p.nsplit = splits;
     return p;
   }
-  // Long ones: two rounds of blocks, of 512 to 4096 positions (a block costs about 5 us next to its
-  // tiles; 64 sequences of 32768 rows: 512 positions 167 us, 4096 139 us; 32 ragged ones of up to
-  // 8191: 512 27 us, 4096 47 us; the sums of more splits than 256 cost more to merge than they save)
-  long long chunk = (units * max_len + 148 * 8 - 1) / (148 * 8);
-  const long long least = units * max_len <= 148 * 4 * kLeast ? kLeast : 512;
-  chunk = std::min<long long>(4096, std::max(least, (chunk + kLeast - 1) / kLeast * kLeast));
+  // Long ones.  One sequence or two: the shortest splits of which two to an SM are all (1 of 131071 rows:
+  // 512 positions 18.9 us, 896 16.8; of 40000: 512 11.6, 384 10.4; 8 heads of 131071: 896 48.0, 3584 45.4;
+  // 2 of up to 65536: 512 19.0, 896 16.5; but 4 ragged ones of up to 32768: 512 21.0, 896 23.6).
+  auto splits_of = [&](long long chunk) { return (max_len + chunk - 1) / chunk; };
+  long long chunk = 0;
+  if (c->batch <= 2) {
+    chunk = std::max(1ll, units * max_len / (148 * 2 * kLeast)) * kLeast;
+    while (chunk <= 4096 && units * splits_of(chunk) > 148 * 2) chunk += kLeast;
+  }
+  // More, which may differ in length: two rounds of blocks, of 512 to 4096 positions (a block costs about
+  // 5 us next to its tiles; 64 sequences of 32768 rows: 512 positions 167 us, 4096 139 us; 32 ragged ones
+  // of up to 8191: 512 27 us, 4096 47 us; the sums of more splits than 256 cost more to merge than they
+  // save)
+  if (chunk == 0 || chunk > (c->batch == 1 ? 4096 : 1024)) {
+    chunk = (units * max_len + 148 * 8 - 1) / (148 * 8);
+    const long long least = units * max_len <= 148 * 4 * kLeast ? kLeast : 512;
+    chunk = std::min<long long>(4096, std::max(least, (chunk + kLeast - 1) / kLeast * kLeast));
+  }
   p.chunk = (int)chunk;
-  p.nsplit = std::max(1, (int)((max_len + chunk - 1) / chunk));
+  p.nsplit = std::max(1, (int)splits_of(chunk));
   p.ml_bytes = p.nsplit > 1 || track ? (size_t)units * p.nsplit * HB * 2 * 4 : 0;
   p.o_bytes = p.nsplit > 1 ? (size_t)units * p.nsplit * HB * c->head_dim * 4 : 0;
   p.score_bytes = track ? (size_t)units * max_len * HB * 4 : 0;
