@@ -11,7 +11,7 @@
 // So the keys are read once and stay in registers (slot order is warp, item, lane: a scan over
 // all slots is one ballot per item and one sum over warps), every pass has one cluster barrier,
 // and the passes end as soon as a digit's rows all stay.  8 x 2 heads of 4160 rows to 4096: 9.4 us;
-// 16 x 2 of 32749 to 2048: 24 us, of which 12 bytes a row are 2 us of HBM time.
+// 16 x 2 of 32749 to 2048: 22 us, of which 12 bytes a row are 2 us of HBM time.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -77,7 +77,8 @@ class Kv4Cache:
         self._lens_shape = torch.Size((b,))
         self._plans = {}
         # what every call needs, looked up once: a call of a decode loop is a few microseconds of host time
-        self._f32, self._i32, self._empty = torch.float32, torch.int32, torch.empty
+        self._f32, self._i32 = torch.float32, torch.int32
+        self._rows = torch.empty(0, device=k_codes.device)  # its new_empty is quicker than torch.empty(device=..)
         self._L, self._raw_stream = lib(), torch._C._cuda_getCurrentRawStream
 
     def _ints(self, t, what):
@@ -120,7 +121,7 @@ class Kv4Cache:
         ``k, v`` f32 ``[B, nkv, n, d]``."""
         if n < 0:
             _refuse(VX_ERR_SHAPE, f"read: {n} rows")
-        k, v = self._empty((2, self.batch, self.n_kv_heads, n, self.head_dim), device=self.device).unbind(0)
+        k, v = self._rows.new_empty((2, self.batch, self.n_kv_heads, n, self.head_dim)).unbind(0)
         if n:
             rc = self._L.vx_kv4_read(self.ctx.h, self._ref, n, self._ints(start, "start"), self._ints(counts, "counts"),
                                      k.data_ptr(), v.data_ptr(), self._raw_stream(self._index))
@@ -147,7 +148,7 @@ class Kv4Cache:
                 self._plans.clear()
             need = self._plans[key] = self._L.vx_kv4_attend_workspace(self._ref, *key)
         out = q.new_empty((batch, width))
-        ws = self._empty(need, device=self.device, dtype=_torch().uint8) if need else None
+        ws = self.k_codes.new_empty(need) if need else None
         rc = self._L.vx_kv4_attend(self.ctx.h, self._ref, q.data_ptr(), q.stride(0) if batch > 1 else width, width // d,
                                    self._ints(lens, "lens"), n, d ** -0.5 if scale is None else scale, track,
                                    out.data_ptr(), width, None if ws is None else ws.data_ptr(), need,

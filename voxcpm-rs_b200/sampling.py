@@ -35,8 +35,8 @@ def sample(ctx: Context, logits, u, temperature=None, top_k=None, top_p=None, mi
 
     ptrs = (values(u, "u"), values(temperature, "temperature"), values(top_k, "top_k", torch.int32),
             values(top_p, "top_p"), values(min_p, "min_p"))
-    ids = torch.empty(rows, device=dev, dtype=torch.int32)
-    lp = torch.empty(rows, device=dev) if return_logprob else None
+    ids = logits.new_empty(rows, dtype=torch.int32)
+    lp = logits.new_empty(rows) if return_logprob else None
     if rows:
         rc = lib().vx_sample(ctx.h, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, *ptrs,
                              ids.data_ptr(), None if lp is None else lp.data_ptr(), raw_stream(ctx.device))
