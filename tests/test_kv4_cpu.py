@@ -121,6 +121,22 @@ def test_strides_of_one_token_or_sequence_do_not_matter(host_cache, monkeypatch)
     assert got == [(0, 0, 1), (0, 128, 3)]
 
 
+def test_outputs_are_f32_whatever_the_default_type(host_cache, monkeypatch):
+    import torch
+    from voxcpm_rs_b200.kv4 import Kv4Cache
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(torch.bfloat16)
+        c = Kv4Cache.from_buffers(_Ctx(), *_bufs())
+        monkeypatch.setattr(c, "_L", type("Lib", (), {"vx_kv4_read": lambda self, *a: 0})())
+        monkeypatch.setattr(c, "_raw_stream", lambda i: 0)
+        assert [t.dtype for t in c.read(3)] == [torch.float32] * 2
+        own = Kv4Cache(_Ctx(), 1, 2, 64, 64)
+        assert own.weights.dtype is torch.float32
+    finally:
+        torch.set_default_dtype(before)
+
+
 def test_plans_do_not_grow_without_end(host_cache, monkeypatch):
     import torch
     monkeypatch.setattr(host_cache, "_L", type("Lib", (), {"vx_kv4_attend_workspace": lambda self, *a: 0,

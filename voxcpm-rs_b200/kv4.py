@@ -44,7 +44,7 @@ class Kv4Cache:
         scales = [torch.zeros(*lead, head_dim // 16, device=dev, dtype=torch.uint8).view(torch.float8_e4m3fn)
                   for _ in range(2)]
         self._hold(ctx, codes[0], scales[0], codes[1], scales[1],
-                   torch.zeros(lead, device=dev) if track else None,
+                   torch.zeros(lead, device=dev, dtype=torch.float32) if track else None,
                    torch.zeros(lead, device=dev, dtype=torch.int64) if track else None)
 
     @classmethod
@@ -78,7 +78,8 @@ class Kv4Cache:
         self._plans = {}
         # what every call needs, looked up once: a call of a decode loop is a few microseconds of host time
         self._f32, self._i32 = torch.float32, torch.int32
-        self._rows = torch.empty(0, device=k_codes.device)  # its new_empty is quicker than torch.empty(device=..)
+        # (its new_empty is quicker than torch.empty(device=..))
+        self._rows = torch.empty(0, device=k_codes.device, dtype=torch.float32)
         self._L, self._raw_stream = lib(), torch._C._cuda_getCurrentRawStream
 
     def _ints(self, t, what):
